@@ -49,6 +49,7 @@ _c = ctypes
 lib = _c.CDLL(LIB_PATH, mode=getattr(os, "RTLD_NOW", 2) | getattr(os, "RTLD_GLOBAL", 0x100))
 
 _vp, _i, _i32p, _f32p, _f64p = _c.c_void_p, _c.c_int, _c.c_void_p, _c.c_void_p, _c.c_void_p
+_i64, _u64, _f = _c.c_int64, _c.c_uint64, _c.c_float
 
 _SIGS = {
     "dn_abi_version": ([], _i),
@@ -93,6 +94,15 @@ _SIGS = {
     "dn_download_tensor": ([_vp, _c.c_char_p, _i, _f32p, _c.c_int64], _i),
     "dn_upload_state": ([_vp, _c.c_char_p, _i, _f32p, _c.c_int64], _i),
     "dn_set_adam_step": ([_vp, _i], _i),
+    "dn_layer_norm_device": ([_vp, _i, _i, _i64, _i, _vp, _i64, _vp, _vp, _f, _vp, _i64, _vp, _vp], _i),
+    "dn_norm_backward_workspace": ([_i64, _i], _i64),
+    "dn_layer_norm_backward_device": ([_vp, _i, _i, _i64, _i, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _vp, _vp,
+                                       _i, _vp, _i64], _i),
+    "dn_dropout_device": ([_vp, _i, _i, _i64, _i64, _vp, _i64, _vp, _i64, _f, _u64, _u64, _vp, _i64], _i),
+    "dn_dropout_add_norm_device": ([_vp, _i, _i, _i, _i64, _i, _vp, _i64, _vp, _i64, _f, _u64, _u64, _vp, _vp, _f, _vp,
+                                    _i64, _vp, _i64, _vp, _vp], _i),
+    "dn_dropout_add_norm_backward_device": ([_vp, _i, _i, _i, _i64, _i, _vp, _i64, _vp, _i64, _vp, _i64, _f, _u64, _u64,
+                                             _vp, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _i, _vp, _i64], _i),
     "dn_tokenizer_parse": ([_vp, _c.c_int64, _c.POINTER(_vp)], _i),
     "dn_tokenizer_free": ([_vp], None),
     "dn_tokenizer_special_ids": ([_vp, _vp, _vp, _vp, _vp], _i),

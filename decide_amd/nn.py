@@ -323,5 +323,69 @@ class Engine:
                                        ctypes.c_void_p(d_C)), self._h)
 
 
+    # The training-block operators (include/decide_hip.h). Arguments named d_*
+    # are raw device addresses, strides are in elements; asynchronous on the
+    # engine's stream. They use the engine's device and stream, not its model.
+
+    def layer_norm_device(self, x_type: str, y_type: str, rows: int, cols: int, d_x: int, ldx: int,
+                          d_w: Optional[int], d_b: Optional[int], eps: float, d_y: int, ldy: int,
+                          d_mean: Optional[int] = None, d_rstd: Optional[int] = None) -> None:
+        """dn_layer_norm_device: y = (x - mean) * rstd * w + b per row; mean and rstd kept when given."""
+        P = native.PRECISIONS
+        check(lib.dn_layer_norm_device(self._h, P[x_type], P[y_type], rows, cols, d_x, ldx, d_w, d_b, eps, d_y, ldy,
+                                       d_mean, d_rstd), self._h)
+
+    @staticmethod
+    def norm_backward_workspace(rows: int, cols: int) -> int:
+        """dn_norm_backward_workspace: bytes of d_work for the two norm backward calls."""
+        n = lib.dn_norm_backward_workspace(rows, cols)
+        if n < 0:
+            raise ValueError(f"norm_backward_workspace: {rows} rows of {cols} columns")
+        return n
+
+    def layer_norm_backward_device(self, dy_type: str, x_type: str, rows: int, cols: int, d_dy: int, lddy: int,
+                                   d_x: int, ldx: int, d_w: Optional[int], d_mean: int, d_rstd: int, d_dx: int,
+                                   lddx: int, d_dw: Optional[int] = None, d_db: Optional[int] = None,
+                                   accumulate: bool = False, d_work: Optional[int] = None,
+                                   work_bytes: int = 0) -> None:
+        """dn_layer_norm_backward_device: dx, and dw / db (= or +=) when given."""
+        P = native.PRECISIONS
+        check(lib.dn_layer_norm_backward_device(self._h, P[dy_type], P[x_type], rows, cols, d_dy, lddy, d_x, ldx, d_w,
+                                                d_mean, d_rstd, d_dx, lddx, d_dw, d_db, bool(accumulate), d_work,
+                                                work_bytes), self._h)
+
+    def dropout_device(self, x_type: str, y_type: str, rows: int, cols: int, d_x: int, ldx: int,
+                       d_res: Optional[int], ldres: int, p: float, seed: int, offset: int, d_y: int,
+                       ldy: int) -> None:
+        """dn_dropout_device: y = [res +] dropout(x); its own gradient with the same p, seed and offset."""
+        P = native.PRECISIONS
+        check(lib.dn_dropout_device(self._h, P[x_type], P[y_type], rows, cols, d_x, ldx, d_res, ldres, p, seed, offset,
+                                    d_y, ldy), self._h)
+
+    def dropout_add_norm_device(self, x_type: str, stream_type: str, y_type: str, rows: int, cols: int, d_x: int,
+                                ldx: int, d_res: int, ldres: int, p: float, seed: int, offset: int,
+                                d_w: Optional[int], d_b: Optional[int], eps: float, d_h: int, ldh: int, d_y: int,
+                                ldy: int, d_mean: Optional[int] = None, d_rstd: Optional[int] = None) -> None:
+        """dn_dropout_add_norm_device: h = res + dropout(x), y = LayerNorm(h)."""
+        P = native.PRECISIONS
+        check(lib.dn_dropout_add_norm_device(self._h, P[x_type], P[stream_type], P[y_type], rows, cols, d_x, ldx,
+                                             d_res, ldres, p, seed, offset, d_w, d_b, eps, d_h, ldh, d_y, ldy, d_mean,
+                                             d_rstd), self._h)
+
+    def dropout_add_norm_backward_device(self, dy_type: str, stream_type: str, dx_type: str, rows: int, cols: int,
+                                         d_dy: int, lddy: int, d_dh: Optional[int], lddh: int, d_h: int, ldh: int,
+                                         p: float, seed: int, offset: int, d_w: Optional[int], d_mean: int,
+                                         d_rstd: int, d_dres: int, lddres: int, d_dx: int, lddx: int,
+                                         d_dw: Optional[int] = None, d_db: Optional[int] = None,
+                                         accumulate: bool = False, d_work: Optional[int] = None,
+                                         work_bytes: int = 0) -> None:
+        """dn_dropout_add_norm_backward_device: dres = dh + LayerNorm'(dy), dx = dropout'(dres), dw, db."""
+        P = native.PRECISIONS
+        check(lib.dn_dropout_add_norm_backward_device(self._h, P[dy_type], P[stream_type], P[dx_type], rows, cols,
+                                                      d_dy, lddy, d_dh, lddh, d_h, ldh, p, seed, offset, d_w, d_mean,
+                                                      d_rstd, d_dres, lddres, d_dx, lddx, d_dw, d_db, bool(accumulate),
+                                                      d_work, work_bytes), self._h)
+
+
 def open_engine(cfg: Config, weights, precision="bf16", device=0) -> Engine:
     return Engine(cfg, weights, precision=precision, device=device)

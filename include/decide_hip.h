@@ -446,6 +446,84 @@ int dn_download_tensor(dn_ctx *ctx, const char *name, int which, float *out, int
 int dn_upload_state(dn_ctx *ctx, const char *name, int which, const float *data, int64_t n);
 int dn_set_adam_step(dn_ctx *ctx, int step);
 
+/* ---- Training-block operators on device arrays ---------------------------
+ * LayerNorm, dropout and the residual boundary made of both, each with its
+ * gradient: what dn_forward_train runs inside the model, as operators of their
+ * own. They need an open context only (no configuration), run asynchronously
+ * on its stream, allocate and wait for nothing, and may be captured into a
+ * graph; replays of graphs that share a d_work must not overlap. The current
+ * device of the calling thread is left as it was.
+ * Arrays are [rows x cols], row r at base + r * ld elements (ld >= cols; any
+ * value for a single row), aligned to their elements: odd widths, strides and
+ * offsets are ordinary. *_type are DN_PRECISION_* codes; the arithmetic and
+ * every sum are fp32, and each output is rounded once. A call's 16-bit arrays are all of one type. Weights, biases,
+ * their gradients and row statistics are fp32. An output may be an input's
+ * very array (the same address, stride and element size); any other overlap
+ * with an output is refused (DN_INVALID_ARG), as are NULL, misaligned or
+ * too-narrow arrays. rows may be 0. Norms take 1 to 32,768 columns
+ * (DN_UNSUPPORTED beyond). No counterpart in the reference, whose model has no
+ * dropout and whose LayerNorm (internal/nn/ops.go:63-138) runs inside it. */
+
+/* y = (x - mean) * rstd * w + b over each row, mean = sum x / cols, rstd =
+ * 1 / sqrt(sum (x - mean)^2 / cols + eps), eps > 0. d_w NULL: 1, d_b NULL: 0.
+ * d_mean and d_rstd ([rows], for the backward pass) may be NULL. x is fp32 or
+ * of y's type. */
+int dn_layer_norm_device(dn_ctx *ctx, int x_type, int y_type, int64_t rows, int cols, const void *d_x, int64_t ldx,
+                         const float *d_w, const float *d_b, float eps, void *d_y, int64_t ldy, float *d_mean,
+                         float *d_rstd);
+
+/* Bytes of d_work for the two backward calls that follow, when they compute a
+ * weight or bias gradient; -1 for sizes they do not take. */
+int64_t dn_norm_backward_workspace(int64_t rows, int cols);
+
+/* The gradients of dn_layer_norm_device from dy, x and the kept mean and rstd:
+ * with xh = (x - mean) * rstd and g = dy * w,
+ *   dx = rstd * (g - mean(g) - xh * mean(g * xh))
+ *   dw = sum over rows of dy * xh,  db = sum over rows of dy
+ * (added to what d_dw and d_db hold when accumulate is set; either may be
+ * NULL). The sums' order depends on the sizes alone: equal calls give equal
+ * bits. x (and dx) is fp32 or of dy's type. */
+int dn_layer_norm_backward_device(dn_ctx *ctx, int dy_type, int x_type, int64_t rows, int cols, const void *d_dy,
+                                  int64_t lddy, const void *d_x, int64_t ldx, const float *d_w, const float *d_mean,
+                                  const float *d_rstd, void *d_dx, int64_t lddx, float *d_dw, float *d_db,
+                                  int accumulate, void *d_work, int64_t work_bytes);
+
+/* y = dropout(x), or res + dropout(x) with d_res (of y's type). With t =
+ * round(65536 * p), an element is kept, and multiplied by 65536 / (65536 - t),
+ * where its 16 random bits are at least t, and is 0 otherwise, whatever it
+ * was. The mask is never stored: the bits are a function of (seed, offset,
+ * row, column) alone, the halves of Philox4x32-10 (Salmon et al., SC'11) with
+ * the seed as its key and (column / 8, row, offset low, offset high) as its
+ * counter: column 8k + 2j + i takes half i (0 low, 1 high) of word j. Calls
+ * that must not share a mask need offsets (or seeds) of their own. The
+ * gradient of x is dn_dropout_device of the gradient of y with the same p,
+ * seed and offset. x and y are of one type or one of them is fp32; at most
+ * 2^34 columns. */
+int dn_dropout_device(dn_ctx *ctx, int x_type, int y_type, int64_t rows, int64_t cols, const void *d_x, int64_t ldx,
+                      const void *d_res, int64_t ldres, float p, uint64_t seed, uint64_t offset, void *d_y,
+                      int64_t ldy);
+
+/* The boundary of two sub-layers in one pass: h = res + dropout(x), rounded to
+ * the stream's type as it is stored, and y = LayerNorm(h) of that. res and h
+ * are of stream_type. Types: all fp32, all of one 16-bit type, or an fp32
+ * stream with a 16-bit y and x of y's type or fp32. p = 0 is the plain
+ * residual. d_h is required (the backward pass reads it). */
+int dn_dropout_add_norm_device(dn_ctx *ctx, int x_type, int stream_type, int y_type, int64_t rows, int cols,
+                               const void *d_x, int64_t ldx, const void *d_res, int64_t ldres, float p,
+                               uint64_t seed, uint64_t offset, const float *d_w, const float *d_b, float eps,
+                               void *d_h, int64_t ldh, void *d_y, int64_t ldy, float *d_mean, float *d_rstd);
+
+/* Its gradients: dres = dh + LayerNorm's gradient of dy (d_dh, the gradient
+ * that reaches h beside the norm, may be NULL), dx = dropout's gradient of the
+ * unrounded dres, dw and db as dn_layer_norm_backward_device. dh and dres are
+ * of stream_type; types as the forward's with dy in x's place and dx in y's. */
+int dn_dropout_add_norm_backward_device(dn_ctx *ctx, int dy_type, int stream_type, int dx_type, int64_t rows, int cols,
+                                        const void *d_dy, int64_t lddy, const void *d_dh, int64_t lddh,
+                                        const void *d_h, int64_t ldh, float p, uint64_t seed, uint64_t offset,
+                                        const float *d_w, const float *d_mean, const float *d_rstd, void *d_dres,
+                                        int64_t lddres, void *d_dx, int64_t lddx, float *d_dw, float *d_db,
+                                        int accumulate, void *d_work, int64_t work_bytes);
+
 #ifdef __cplusplus
 }
 #endif
