@@ -4,12 +4,12 @@
 
 #include <stdint.h>
 
-// Widest row of the norms: 1,024 threads hold it in registers, 32 elements each.
-constexpr int kNormMaxCols = 32768;
+// Widest row of the norms: 1,024 threads hold it in registers, 16 elements each.
+constexpr int kNormMaxCols = 16384;
 
 // A dropout mask: the element in column c of row r is kept where its 16
-// random bits (mask_bits) are at least `threshold`, and scaled by `scale` =
-// 65536 / (65536 - threshold). threshold 0 keeps every element unscaled.
+// random bits are at least `threshold`, and scaled by `scale` = 65536 / (65536
+// - threshold). threshold 0 keeps every element unscaled, 65536 none.
 struct DropMask {
   uint32_t threshold;
   float scale;

@@ -21,7 +21,7 @@ struct Refusal {
 constexpr int64_t kMaxRows = 0x7fffffff;
 // Columns of the elementwise dropout: the mask's counter holds a block of
 // eight columns in 32 bits.
-constexpr int64_t kMaxDropCols = (int64_t)1 << 34;
+constexpr int64_t kMaxDropCols = ((int64_t)1 << 34) - 8;
 
 inline bool known(int t) { return t == DN_PRECISION_FP32 || t == DN_PRECISION_BF16 || t == DN_PRECISION_FP16; }
 inline int width(int t) { return t == DN_PRECISION_FP32 ? 4 : 2; }
@@ -63,20 +63,21 @@ inline bool apart(const Array &a, const Array &b) {
   return d >= a.cols * a.es && d + b.cols * b.es <= sa;
 }
 
+inline std::string said(const char *op) { return std::string("decide_hip: ") + op + ": "; }
+
 inline Refusal arrays(const char *op, const Array *v, int n) {
-  const std::string pre = std::string("decide_hip: ") + op + ": ";
   for (int i = 0; i < n; i++) {
     const Array &a = v[i];
     if (a.rows == 0 || a.cols == 0) continue;
     if (!a.p) {
-      if (a.required) return {DN_INVALID_ARG, pre + a.name + " is NULL"};
+      if (a.required) return {DN_INVALID_ARG, said(op) + a.name + " is NULL"};
       continue;
     }
-    if ((uintptr_t)a.p % a.es) return {DN_INVALID_ARG, pre + a.name + " is not aligned to its elements"};
+    if ((uintptr_t)a.p % a.es) return {DN_INVALID_ARG, said(op) + a.name + " is not aligned to its elements"};
     if (a.ld < 0 || (a.rows > 1 && a.ld < a.cols))
-      return {DN_INVALID_ARG, pre + "the row stride of " + a.name + " is less than its columns"};
+      return {DN_INVALID_ARG, said(op) + "the row stride of " + a.name + " is less than its columns"};
     if (a.rows > 1 && a.ld > ((int64_t)1 << 56) / a.rows)
-      return {DN_INVALID_ARG, pre + "the row stride of " + a.name + " passes the address range"};
+      return {DN_INVALID_ARG, said(op) + "the row stride of " + a.name + " passes the address range"};
   }
   for (int i = 0; i < n; i++)
     for (int j = i + 1; j < n; j++) {
@@ -84,30 +85,28 @@ inline Refusal arrays(const char *op, const Array *v, int n) {
       if (!a.p || !b.p || !(a.out || b.out) || a.rows == 0 || a.cols == 0 || b.rows == 0 || b.cols == 0) continue;
       const bool same = a.p == b.p && a.es == b.es && (a.ld == b.ld || a.rows == 1) && a.matrix && b.matrix;
       if (same && a.out != b.out) continue;  // in place
-      if (!apart(a, b)) return {DN_INVALID_ARG, pre + a.name + " overlaps " + b.name};
+      if (!apart(a, b)) return {DN_INVALID_ARG, said(op) + a.name + " overlaps " + b.name};
     }
   return {};
 }
 
 inline Refusal sizes(const char *op, int64_t rows, int64_t cols, int64_t min_cols, int64_t max_cols) {
-  const std::string pre = std::string("decide_hip: ") + op + ": ";
-  if (rows < 0 || cols < min_cols) return {DN_INVALID_ARG, pre + "bad number of rows or columns"};
+  if (rows < 0 || cols < min_cols) return {DN_INVALID_ARG, said(op) + "bad number of rows or columns"};
   if (rows > kMaxRows || cols > max_cols)
-    return {DN_UNSUPPORTED, pre + "at most 2147483647 rows and " + std::to_string(max_cols) + " columns"};
+    return {DN_UNSUPPORTED, said(op) + "at most 2147483647 rows and " + std::to_string(max_cols) + " columns"};
   return {};
 }
 
 inline Refusal types(const char *op, bool all_known, bool built) {
-  const std::string pre = std::string("decide_hip: ") + op + ": ";
-  if (!all_known) return {DN_INVALID_ARG, pre + "unknown precision"};
-  if (!built) return {DN_UNSUPPORTED, pre + "this combination of types is not built"};
+  if (!all_known) return {DN_INVALID_ARG, said(op) + "unknown precision"};
+  if (!built) return {DN_UNSUPPORTED, said(op) + "this combination of types is not built"};
   return {};
 }
 
 // The mask of a dropout probability: threshold = p in units of 2^-16, to nearest.
 inline Refusal mask(const char *op, float p, uint64_t seed, uint64_t offset, DropMask *m) {
   if (!(p >= 0.0f && p <= 1.0f))
-    return {DN_INVALID_ARG, std::string("decide_hip: ") + op + ": the dropout probability is not in [0, 1]"};
+    return {DN_INVALID_ARG, said(op) + "the dropout probability is not in [0, 1]"};
   m->threshold = (uint32_t)std::nearbyint((double)p * 65536.0);
   m->scale = m->threshold < 65536 ? (float)(65536.0 / (65536 - m->threshold)) : 0.0f;
   m->k0 = (uint32_t)seed;
@@ -119,7 +118,7 @@ inline Refusal mask(const char *op, float p, uint64_t seed, uint64_t offset, Dro
 
 inline Refusal epsilon(const char *op, float eps) {
   if (!(eps > 0.0f) || !std::isfinite(eps))
-    return {DN_INVALID_ARG, std::string("decide_hip: ") + op + ": eps is not a positive number"};
+    return {DN_INVALID_ARG, said(op) + "eps is not a positive number"};
   return {};
 }
 
@@ -149,7 +148,7 @@ inline Refusal norm_grad(int dy_type, int x_type, const NormGradArgs &a, int64_t
   BLOCKCHK(types(op, known(dy_type) && known(x_type), norm_types_ok(x_type, dy_type)));
   BLOCKCHK(sizes(op, a.rows, a.cols, 1, kNormMaxCols));
   const int64_t R = a.rows, C = a.cols, W = a.dw || a.db ? work_floats : 0;
-  if (work_bytes < 4 * W) return {DN_INVALID_ARG, std::string("decide_hip: ") + op + ": the workspace is too small"};
+  if (work_bytes < 4 * W) return {DN_INVALID_ARG, said(op) + "the workspace is too small"};
   const Array v[] = {{"dy", a.dy, R, C, a.lddy, width(dy_type), false, true, true},
                      {"x", a.h, R, C, a.ldh, width(x_type), false, true, true},
                      {"w", a.w, 1, C, C, 4, false, false, false},
@@ -202,7 +201,7 @@ inline Refusal boundary_grad(int dy_type, int stream_type, int dx_type, float p,
   BLOCKCHK(sizes(op, a->rows, a->cols, 1, kNormMaxCols));
   BLOCKCHK(mask(op, p, seed, offset, &a->mask));
   const int64_t R = a->rows, C = a->cols, W = a->dw || a->db ? work_floats : 0;
-  if (work_bytes < 4 * W) return {DN_INVALID_ARG, std::string("decide_hip: ") + op + ": the workspace is too small"};
+  if (work_bytes < 4 * W) return {DN_INVALID_ARG, said(op) + "the workspace is too small"};
   const Array v[] = {{"dy", a->dy, R, C, a->lddy, width(dy_type), false, true, true},
                      {"dh", a->dh, R, C, a->lddh, width(stream_type), false, false, true},
                      {"h", a->h, R, C, a->ldh, width(stream_type), false, true, true},

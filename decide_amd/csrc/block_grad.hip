@@ -6,125 +6,193 @@
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kRowParts = 256;  // partial sums of the weight gradients
+#ifndef GRAD_PARTS
+#define GRAD_PARTS 512
+#endif
+#ifndef WIDE_PARTS
+#define WIDE_PARTS 256
+#endif
+// Most partial sums of the weight gradients (and workgroups of their kernel).
+constexpr int kMaxParts = GRAD_PARTS;
 
-__device__ __forceinline__ float block_sum(float v, float *lds) {
-#pragma unroll
-  for (int m = 32; m > 0; m >>= 1) v += __shfl_xor(v, m);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
-  __syncthreads();
-  float s = 0;
-#pragma unroll
-  for (int i = 0; i < kThreads / 64; i++) s += lds[i];
-  return s;
+template <int LPR>
+int row_parts(int64_t rows) {
+  constexpr int groups = row_threads(LPR) / LPR;
+  return (int)std::min<int64_t>(LPR > 128 ? WIDE_PARTS : kMaxParts, (rows + groups - 1) / groups);
 }
 
-int row_parts(int64_t rows) { return (int)std::min<int64_t>(kRowParts, (rows + 7) / 8); }
-
-// The input gradients, one workgroup per row: with xh = (h - mean) rstd and
-// g = dy w, dres = dh + rstd (g - mean(g) - xh mean(g xh)) and dx = dropout's
-// gradient of it (the forward's mask and scale), from the unrounded sum.
-template <class D, class S, class X, bool BOUNDARY>
-__global__ __launch_bounds__(kThreads) void norm_grad_kernel(NormGradArgs a) {
-  __shared__ float lds[kThreads / 64];
-  const int blocks = (a.cols + 7) / 8;
-  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+// All gradients in one pass over rows held in registers (LPR threads per row,
+// VPT blocks of eight columns each): with xh = (h - mean) rstd and g = dy w,
+// dres = dh + rstd (g - mean(g) - xh mean(g xh)) and dx = dropout's gradient of
+// it (the forward's mask and scale), from the unrounded sum. Each thread adds
+// dy xh and dy of its columns over its rows; a workgroup's sums go to its
+// slice of the workspace, [2][cols].
+template <class D, class S, class X, bool BOUNDARY, int VEC, int LPR, int VPT>
+__global__ __launch_bounds__(row_threads(LPR)) void norm_grad_kernel(NormGradArgs a) {
+  constexpr int GROUPS = row_threads(LPR) / LPR, W = LPR > 64 ? LPR / 64 : 1;
+  __shared__ float slots[2][2 * W];
+  const int lane = threadIdx.x % LPR, cols = a.cols;
+  const float inv = 1.0f / (float)cols;
+  float sw[VPT][VEC], sb[VPT][VEC];
+#pragma unroll
+  for (int j = 0; j < VPT; j++)
+#pragma unroll
+    for (int i = 0; i < VEC; i++) sw[j][i] = 0.0f, sb[j][i] = 0.0f;
+  int turn = 0;
+  for (int64_t row = row_of<LPR>((int64_t)blockIdx.x * GROUPS); row < a.rows;
+       row += (int64_t)gridDim.x * GROUPS, turn ^= 1) {
+    // The weights are read again for every row (from the caches): held, they
+    // would cost the registers of a wave per SIMD.
+    const float *weight = a.w;
+    asm volatile("" : "+s"(weight));
+    Raw<S, VEC> h[VPT], dh[BOUNDARY ? VPT : 1];
+    Raw<D, VEC> dy[VPT];
+#pragma unroll
+    for (int j = 0; j < VPT; j++) {
+      const int c = VEC * (lane + j * LPR);
+      h[j] = fetch<S, VEC>((const S *)a.h + row * a.ldh, c, cols);
+      dy[j] = fetch<D, VEC>((const D *)a.dy + row * a.lddy, c, cols);
+    }
+    if constexpr (BOUNDARY)
+      if (a.dh)
+#pragma unroll
+        for (int j = 0; j < VPT; j++)
+          dh[j] = fetch<S, VEC>((const S *)a.dh + row * a.lddh, VEC * (lane + j * LPR), cols);
     const float mean = a.mean[row], rstd = a.rstd[row];
-    auto terms = [&](int k, int n, float(&g)[8], float(&xh)[8]) {
-      float w[8];
-      load8((const D *)a.dy + row * a.lddy + 8 * k, n, g);
-      load8((const S *)a.h + row * a.ldh + 8 * k, n, xh);
-      if (a.w) load8(a.w + 8 * k, n, w);
+    float g[VPT][VEC], xh[VPT][VEC];
+    float s[2] = {0.0f, 0.0f};
 #pragma unroll
-      for (int j = 0; j < 8; j++) {
-        xh[j] = j < n ? (xh[j] - mean) * rstd : 0.0f;
-        g[j] *= a.w ? w[j] : 1.0f;
-      }
-    };
-    float s1 = 0, s2 = 0;
-    for (int k = threadIdx.x; k < blocks; k += kThreads) {
-      float g[8], xh[8];
-      terms(k, a.cols - 8 * k, g, xh);
+    for (int j = 0; j < VPT; j++) {
+      const int c = VEC * (lane + j * LPR);
+      float w[VEC];
 #pragma unroll
-      for (int j = 0; j < 8; j++) {
-        s1 += g[j];
-        s2 += g[j] * xh[j];
+      for (int i = 0; i < VEC; i++) w[i] = 1.0f;
+      if (weight) load<float, VEC>(weight, c, cols, w);
+      unpack<S, VEC>(h[j], cols - c, xh[j]);
+      unpack<D, VEC>(dy[j], cols - c, g[j]);
+#pragma unroll
+      for (int i = 0; i < VEC; i++) {
+        // Columns past the row hold dy = 0.
+        xh[j][i] = (xh[j][i] - mean) * rstd;
+        sw[j][i] += g[j][i] * xh[j][i];
+        sb[j][i] += g[j][i];
+        g[j][i] *= w[i];
+        s[0] += g[j][i];
+        s[1] += g[j][i] * xh[j][i];
       }
     }
-    const float c1 = block_sum(s1, lds) / (float)a.cols, c2 = block_sum(s2, lds) / (float)a.cols;
-    for (int k = threadIdx.x; k < blocks; k += kThreads) {
-      const int n = a.cols - 8 * k;
-      float g[8], xh[8];
-      terms(k, n, g, xh);
+    row_sum<LPR>(s, slots[turn]);
+    const float c1 = mul_rounded(s[0], inv), c2 = mul_rounded(s[1], inv);
 #pragma unroll
-      for (int j = 0; j < 8; j++) g[j] = rstd * (g[j] - c1 - xh[j] * c2);
-      if constexpr (BOUNDARY) {
+    for (int j = 0; j < VPT; j++) {
+      const int c = VEC * (lane + j * LPR);
+#pragma unroll
+      for (int i = 0; i < VEC; i++) g[j][i] = rstd * (g[j][i] - c1 - xh[j][i] * c2);
+      if constexpr (BOUNDARY)
         if (a.dh) {
-          float r[8];
-          load8((const S *)a.dh + row * a.lddh + 8 * k, n, r);
+          float r[VEC];
+          unpack<S, VEC>(dh[j], cols - c, r);
 #pragma unroll
-          for (int j = 0; j < 8; j++) g[j] = r[j] + g[j];
+          for (int i = 0; i < VEC; i++) g[j][i] += r[i];
         }
-      }
-      store8((S *)a.dres + row * a.lddres + 8 * k, n, g);
-      if constexpr (BOUNDARY) {
-        drop8(a.mask, (uint32_t)row, k, g);
-        store8((X *)a.dx + row * a.lddx + 8 * k, n, g);
-      }
+      store<S, VEC>((S *)a.dres + row * a.lddres, c, cols, g[j]);
+    }
+    if constexpr (BOUNDARY) {
+      Columns<LPR, VPT, VEC>::drop(a.mask, (uint32_t)row, lane, cols, g);
+#pragma unroll
+      for (int j = 0; j < VPT; j++) store<X, VEC>((X *)a.dx + row * a.lddx, VEC * (lane + j * LPR), cols, g[j]);
     }
   }
+  if (!a.work) return;
+  float *out = a.work + (int64_t)blockIdx.x * 2 * cols;
+  if constexpr (LPR > 64) {
+#pragma unroll
+    for (int j = 0; j < VPT; j++) {
+      const int c = VEC * (lane + j * LPR);
+      store<float, VEC>(out, c, cols, sw[j]);
+      store<float, VEC>(out + cols, c, cols, sb[j]);
+    }
+  } else {
+    // Rows of one wave in registers, then the four waves through LDS in order.
+    constexpr int WAVES = kThreads / 64, COLS = LPR * VPT * VEC;
+    __shared__ float part[WAVES][COLS];
+    auto join = [&](float(&v)[VPT][VEC], float *to) {
+#pragma unroll
+      for (int j = 0; j < VPT; j++)
+#pragma unroll
+        for (int i = 0; i < VEC; i++) {
+#pragma unroll
+          for (int m = LPR; m < 64; m <<= 1) v[j][i] += __shfl_xor(v[j][i], m);
+        }
+      if ((threadIdx.x & 63) < LPR)
+#pragma unroll
+        for (int j = 0; j < VPT; j++)
+#pragma unroll
+          for (int i = 0; i < VEC; i++) part[threadIdx.x >> 6][VEC * (lane + j * LPR) + i] = v[j][i];
+      __syncthreads();
+      for (int c = threadIdx.x; c < cols; c += kThreads) {
+        float t = 0;
+#pragma unroll
+        for (int k = 0; k < WAVES; k++) t += part[k][c];
+        to[c] = t;
+      }
+      __syncthreads();
+    };
+    join(sw, out);
+    join(sb, out + cols);
+  }
 }
 
-// Partial sums over every gridDim.y-th row: work[part][0][c] = sum dy xh,
-// work[part][1][c] = sum dy.
-template <class D, class S>
-__global__ __launch_bounds__(kThreads) void norm_sums_kernel(NormGradArgs a) {
-  const int c = blockIdx.x * kThreads + threadIdx.x;
-  if (c >= a.cols) return;
-  float sw = 0, sb = 0;
-  for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
-    const float dy = (float)((const D *)a.dy)[row * a.lddy + c];
-    const float h = (float)((const S *)a.h)[row * a.ldh + c];
-    sw += dy * ((h - a.mean[row]) * a.rstd[row]);
-    sb += dy;
+// The workgroups' sums in order: blockIdx.y 0 dw, 1 db; 16 columns of a
+// workgroup, 64 threads each, whose loads are made eight at a time.
+__global__ __launch_bounds__(1024) void norm_join_kernel(NormGradArgs a, int parts) {
+  constexpr int COLS = 16, SPLIT = 1024 / COLS, BATCH = 8;
+  __shared__ float lds[SPLIT][COLS + 1];
+  float *to = blockIdx.y ? a.db : a.dw;
+  if (!to) return;
+  const int i = threadIdx.x % COLS, c = blockIdx.x * COLS + i, k = threadIdx.x / COLS;
+  const float *from = a.work + (int64_t)blockIdx.y * a.cols + min(c, a.cols - 1);
+  float s = 0;
+  for (int p = k; p < parts; p += SPLIT * BATCH) {
+    float v[BATCH];
+#pragma unroll
+    for (int j = 0; j < BATCH; j++) v[j] = from[(int64_t)min(p + j * SPLIT, parts - 1) * 2 * a.cols];
+#pragma unroll
+    for (int j = 0; j < BATCH; j++) s += p + j * SPLIT < parts ? v[j] : 0.0f;
   }
-  float *out = a.work + (int64_t)blockIdx.y * 2 * a.cols;
-  out[c] = sw;
-  out[a.cols + c] = sb;
-}
-
-__global__ __launch_bounds__(kThreads) void norm_sums_join_kernel(NormGradArgs a, int parts) {
-  const int c = blockIdx.x * kThreads + threadIdx.x;
-  if (c >= a.cols) return;
-  float sw = 0, sb = 0;
-  for (int p = 0; p < parts; p++) {
-    sw += a.work[(int64_t)p * 2 * a.cols + c];
-    sb += a.work[((int64_t)p * 2 + 1) * a.cols + c];
+  lds[k][i] = s;
+  __syncthreads();
+  if (k < 8) {
+    s = 0;
+#pragma unroll
+    for (int j = 0; j < SPLIT / 8; j++) s += lds[k * (SPLIT / 8) + j][i];
+    lds[k * (SPLIT / 8)][i] = s;
   }
-  if (a.dw) a.dw[c] = a.accumulate ? a.dw[c] + sw : sw;
-  if (a.db) a.db[c] = a.accumulate ? a.db[c] + sb : sb;
+  __syncthreads();
+  if (k == 0 && c < a.cols) {
+    s = 0;
+#pragma unroll
+    for (int j = 0; j < 8; j++) s += lds[j * (SPLIT / 8)][i];
+    to[c] = a.accumulate ? to[c] + s : s;
+  }
 }
 
 template <class D, class S, class X, bool BOUNDARY>
-hipError_t grad_launch(const NormGradArgs &a, hipStream_t s) {
-  const int parts = row_parts(a.rows);
-  const unsigned cb = (unsigned)((a.cols + kThreads - 1) / kThreads);
-  if (a.dw || a.db) {
-    // The sums first: dres may be written over dy or h.
-    if (parts > 0) {
-      hipLaunchKernelGGL((norm_sums_kernel<D, S>), dim3(cb, parts), dim3(kThreads), 0, s, a);
-      const hipError_t e = hipGetLastError();
-      if (e != hipSuccess) return e;
+hipError_t grad_launch(const NormGradArgs &args, hipStream_t s) {
+  return with_row_shape<vec_of<D, S, X>>(args.cols, [&](auto vec, auto lpr, auto vpt) {
+    constexpr int VEC = vec, LPR = lpr, VPT = vpt, THREADS = row_threads(LPR);
+    NormGradArgs a = args;
+    const int parts = row_parts<LPR>(a.rows);
+    if (!a.dw && !a.db) a.work = nullptr;
+    if (parts > 0)
+      hipLaunchKernelGGL((norm_grad_kernel<D, S, X, BOUNDARY, VEC, LPR, VPT>), dim3(parts), dim3(THREADS), 0, s, a);
+    hipError_t e = hipGetLastError();
+    if (e == hipSuccess && (a.dw || a.db)) {
+      hipLaunchKernelGGL(norm_join_kernel, dim3((a.cols + 15) / 16, a.db ? 2 : 1), dim3(1024), 0, s, a, parts);
+      e = hipGetLastError();
     }
-    hipLaunchKernelGGL(norm_sums_join_kernel, dim3(cb), dim3(kThreads), 0, s, a, parts);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-  }
-  if (a.rows == 0) return hipSuccess;
-  hipLaunchKernelGGL((norm_grad_kernel<D, S, X, BOUNDARY>), dim3((unsigned)std::min<int64_t>(a.rows, 1 << 20)),
-                     dim3(kThreads), 0, s, a);
-  return hipGetLastError();
+    return e;
+  });
 }
 
 template <class T>
@@ -144,7 +212,17 @@ hipError_t boundary_grad_pick(int dy_type, int stream_type, int dx_type, const N
 
 }  // namespace
 
-int64_t norm_grad_work(int64_t rows, int cols) { return (int64_t)row_parts(rows) * 2 * cols; }
+// The larger of what calls with and without an fp32 array use.
+int64_t norm_grad_work(int64_t rows, int cols) {
+  int parts = 0;
+  auto most = [&](auto, auto lpr, auto) {
+    parts = std::max(parts, row_parts<lpr>(rows));
+    return hipSuccess;
+  };
+  (void)with_row_shape<4>(cols, most);
+  (void)with_row_shape<8>(cols, most);
+  return (int64_t)parts * 2 * cols;
+}
 
 hipError_t launch_norm_grad(int dy_type, int x_type, const NormGradArgs &a, hipStream_t s) {
   return dy_type == PREC_F16 ? norm_grad_pick<f16>(dy_type, x_type, a, s) : norm_grad_pick<bf16>(dy_type, x_type, a, s);

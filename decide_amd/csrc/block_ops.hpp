@@ -4,6 +4,8 @@
 // gradients.
 #pragma once
 
+#include <type_traits>
+
 #include "block_args.hpp"
 #include "common.hpp"
 
@@ -22,12 +24,13 @@ hipError_t launch_dropout(int x_type, int y_type, const DropArgs &a, hipStream_t
 // as 1, 2, 3", SC'11): ten rounds of two 32 x 32 -> 64-bit products, the
 // published multipliers and key increments.
 __device__ __forceinline__ uint4 philox(uint32_t c0, uint32_t c1, uint32_t c2, uint32_t c3, uint32_t k0, uint32_t k1) {
+  auto xor3 = [](uint32_t x, uint32_t y, uint32_t z) { return __builtin_amdgcn_bitop3_b32(x, y, z, 0x96); };
 #pragma unroll
   for (int i = 0; i < 10; i++) {
     const uint64_t a = (uint64_t)c0 * 0xD2511F53u, b = (uint64_t)c2 * 0xCD9E8D57u;
-    c0 = (uint32_t)(b >> 32) ^ c1 ^ k0;
+    c0 = xor3((uint32_t)(b >> 32), c1, k0);
     c1 = (uint32_t)b;
-    c2 = (uint32_t)(a >> 32) ^ c3 ^ k1;
+    c2 = xor3((uint32_t)(a >> 32), c3, k1);
     c3 = (uint32_t)a;
     k0 += 0x9E3779B9u;
     k1 += 0xBB67AE85u;
@@ -35,48 +38,247 @@ __device__ __forceinline__ uint4 philox(uint32_t c0, uint32_t c1, uint32_t c2, u
   return make_uint4(c0, c1, c2, c3);
 }
 
-// Drops the elements of columns 8 * block .. 8 * block + 7 of a row in place:
-// one generator block gives their eight 16-bit draws. A dropped element is 0
-// whatever it was (also an infinity or a NaN), so it is selected, not multiplied.
-__device__ __forceinline__ void drop8(const DropMask &m, uint32_t row, uint32_t block, float (&v)[8]) {
-  if (m.threshold == 0) return;
-  const uint4 r = philox(block, row, m.o0, m.o1, m.k0, m.k1);
-  const uint32_t word[4] = {r.x, r.y, r.z, r.w};
+// Drops elements in place, from the generator's words that hold their 16-bit
+// draws: element j takes half j % 2 (0 low) of word j / 2. A dropped element
+// is 0 whatever it was (also an infinity or a NaN), so it is selected, not
+// multiplied. A half is at least the threshold t > 0 where its word, with that
+// half in the upper bits, is above 65536 t - 1: the lower bits only add, and
+// at t = 65536 nothing is above 2^32 - 1.
+__device__ __forceinline__ float keep_scaled(const DropMask &m, uint32_t upper, float v) {
+  return upper > (m.threshold << 16) - 1u ? v * m.scale : 0.0f;
+}
+template <int N>
+__device__ __forceinline__ void drop_by(const DropMask &m, const uint32_t (&word)[N / 2], float (&v)[N]) {
 #pragma unroll
-  for (int j = 0; j < 4; j++) {
-    v[2 * j] = (word[j] & 0xffffu) >= m.threshold ? v[2 * j] * m.scale : 0.0f;
-    v[2 * j + 1] = (word[j] >> 16) >= m.threshold ? v[2 * j + 1] * m.scale : 0.0f;
+  for (int j = 0; j < N / 2; j++) {
+    v[2 * j] = keep_scaled(m, word[j] << 16, v[2 * j]);
+    v[2 * j + 1] = keep_scaled(m, word[j], v[2 * j + 1]);
   }
 }
 
-// Eight consecutive elements from an address aligned to the element only: the
-// hardware takes 16-byte accesses at any element's alignment, so odd row
-// strides need no variant of their own. n < 8 (a row's last, partial block):
-// element by element, zeros past n.
+// The columns of a row that one of its LPR threads holds: VPT vectors of VEC,
+// vector j at column VEC * (lane + j * LPR).
+template <int LPR, int VPT, int VEC>
+struct Columns {
+  // The elements of a row of `cols` dropped in place. One generator block covers
+  // eight columns: a vector of eight, or the vectors of four of two neighbouring
+  // lanes, or a row of less than eight columns with one lane each. The two
+  // lanes share the work: of vectors j and j + 1 the even lane generates j's
+  // block and the odd one j + 1's, and each hands the other its half. They skip
+  // a vector together, when the even lane's starts past the row.
+  static __device__ __forceinline__ void drop(const DropMask &m, uint32_t row, int lane, int cols,
+                                              float (&v)[VPT][VEC]) {
+    if (m.threshold == 0) return;
+    if constexpr (VEC == 8) {
+#pragma unroll
+      for (int j = 0; j < VPT; j++) {
+        const int block = lane + j * LPR;
+        if (j > 0 && 8 * block >= cols) break;
+        const uint4 r = philox((uint32_t)block, row, m.o0, m.o1, m.k0, m.k1);
+        const uint32_t word[4] = {r.x, r.y, r.z, r.w};
+        drop_by<8>(m, word, v[j]);
+      }
+    } else if constexpr (VEC == 1) {
+      const uint4 r = philox(0, row, m.o0, m.o1, m.k0, m.k1);
+      const uint32_t word = lane < 4 ? (lane < 2 ? r.x : r.y) : (lane < 6 ? r.z : r.w);
+      v[0][0] = keep_scaled(m, lane & 1 ? word : word << 16, v[0][0]);
+    } else {
+      const bool odd = lane & 1;
+#pragma unroll
+      for (int j = 0; j < VPT; j += 2) {
+        const bool pair = j + 1 < VPT;
+        if (j > 0 && 4 * ((lane & ~1) + j * LPR) >= cols) break;
+        const uint4 r = philox((uint32_t)(lane + (j + (pair && odd ? 1 : 0)) * LPR) >> 1, row, m.o0, m.o1, m.k0, m.k1);
+        const uint32_t low[2] = {r.x, r.y}, high[2] = {r.z, r.w};
+        uint32_t mine[2], other[2];
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+          mine[i] = odd ? high[i] : low[i];
+          if (pair) other[i] = dpp_u32<0xB1>(odd ? low[i] : high[i]);  // the neighbour's: quad_perm 1,0,3,2
+        }
+        if (pair) {
+          uint32_t first[2], second[2];
+#pragma unroll
+          for (int i = 0; i < 2; i++) {
+            first[i] = odd ? other[i] : mine[i];
+            second[i] = odd ? mine[i] : other[i];
+          }
+          drop_by<4>(m, first, v[j]);
+          drop_by<4>(m, second, v[j + 1 < VPT ? j + 1 : j]);
+        } else {
+          drop_by<4>(m, mine, v[j]);
+        }
+      }
+    }
+  }
+};
+
+// VEC consecutive elements of a row as they lie in memory. The address needs
+// the elements' alignment only: the hardware takes accesses of up to 16 bytes
+// at any address, so odd strides and offsets need no variant of their own.
+template <class T, int VEC>
+struct Raw {
+  uint32_t q[VEC * sizeof(T) / 4];
+  __device__ __forceinline__ float at(int j) const {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(q[j]);
+    else return j & 1 ? hi16<T>(q[j / 2]) : lo16<T>(q[j / 2]);
+  }
+};
 template <class T>
-__device__ __forceinline__ void load8(const T *p, int n, float (&v)[8]) {
-  if (n >= 8) {
-    T t[8];
-    __builtin_memcpy(t, p, sizeof(t));
+struct Raw<T, 1> {
+  T q;
+  __device__ __forceinline__ float at(int) const { return (float)q; }
+};
+
+// Columns c .. c + VEC - 1 of a row of cols >= VEC. Where those pass the row's
+// end (its last, partial vector, and threads past it) the VEC elements that end
+// with the row are read instead, so that every lane makes the same loads and no
+// branch stands between them; unpack moves them into place.
+template <class T, int VEC>
+__device__ __forceinline__ Raw<T, VEC> fetch(const T *row, int c, int cols) {
+  Raw<T, VEC> r;
+  __builtin_memcpy(&r, row + (unsigned)min(c, cols - VEC), sizeof(r));
+  return r;
+}
+
+// The vector's elements as floats, zeros past the row. n: columns from c on.
+template <class T, int VEC>
+__device__ __forceinline__ void unpack(const Raw<T, VEC> &r, int n, float (&v)[VEC]) {
 #pragma unroll
-    for (int j = 0; j < 8; j++) v[j] = (float)t[j];
-  } else {
+  for (int j = 0; j < VEC; j++) v[j] = r.at(j);
+  if (n < VEC) {
+    const int by = VEC - max(n, 0);  // elements down, 1 .. VEC
 #pragma unroll
-    for (int j = 0; j < 8; j++) v[j] = j < n ? (float)p[j] : 0.0f;
+    for (int step = VEC; step > 0; step >>= 1)
+#pragma unroll
+      for (int j = 0; j < VEC; j++) v[j] = by & step ? (j + step < VEC ? v[j + step] : 0.0f) : v[j];
   }
 }
-template <class T>
-__device__ __forceinline__ void store8(T *p, int n, const float (&v)[8]) {
-  if (n >= 8) {
-    T t[8];
+
+template <class T, int VEC>
+__device__ __forceinline__ void load(const T *row, int c, int cols, float (&v)[VEC]) {
+  unpack<T, VEC>(fetch<T, VEC>(row, c, cols), cols - c, v);
+}
+
+template <class T, int VEC>
+__device__ __forceinline__ void store(T *row, int c, int cols, const float (&v)[VEC]) {
+  if (cols - c >= VEC) {
+    T t[VEC];
 #pragma unroll
-    for (int j = 0; j < 8; j++) t[j] = to_elem<T>(v[j]);
-    __builtin_memcpy(p, t, sizeof(t));
-  } else {
+    for (int j = 0; j < VEC; j++) t[j] = to_elem<T>(v[j]);
+    __builtin_memcpy(row + (unsigned)c, t, sizeof(t));
+  } else if (c < cols) {
+    asm volatile("");  // keeps the compiler from splitting the store above to share its parts with these
 #pragma unroll
-    for (int j = 0; j < 8; j++)
-      if (j < n) p[j] = to_elem<T>(v[j]);
+    for (int j = 0; j < VEC - 1; j++)
+      if (c + j < cols) row[(unsigned)(c + j)] = to_elem<T>(v[j]);
   }
 }
+
+// The sum of each v[i] over the LPR consecutive threads that share a row, in
+// all of them: DPP moves within 16 lanes and row swaps across them (no LDS
+// round trips: 10 dependent steps of ~8 cycles where a shuffle takes ~60), and
+// for a row over several waves one exchange through LDS. The order of the sum
+// depends on LPR alone. `slot`: LDS that no other reduction of the same loop
+// iteration uses, so that one barrier per reduction is enough.
+template <int LPR, int N>
+__device__ __forceinline__ void row_sum(float (&v)[N], float *slot) {
+  auto add = [&](auto move) {
+#pragma unroll
+    for (int i = 0; i < N; i++) v[i] += __uint_as_float(move(__float_as_uint(v[i])));
+  };
+  add([](unsigned x) { return dpp_u32<0xB1>(x); });  // quad_perm 1,0,3,2
+  add([](unsigned x) { return dpp_u32<0x4E>(x); });  // quad_perm 2,3,0,1
+  add([](unsigned x) { return dpp_u32<0x141>(x); });  // row_half_mirror
+  if constexpr (LPR >= 16) add([](unsigned x) { return dpp_u32<0x140>(x); });  // row_mirror
+  if constexpr (LPR >= 32)
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v[i]), __float_as_uint(v[i]), false, false);
+      v[i] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+  if constexpr (LPR >= 64)
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[i]), __float_as_uint(v[i]), false, false);
+      v[i] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+  if constexpr (LPR > 64) {
+    constexpr int W = LPR / 64;
+    if ((threadIdx.x & 63) == 0)
+#pragma unroll
+      for (int i = 0; i < N; i++) slot[i * W + (threadIdx.x >> 6)] = v[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      v[i] = 0;
+#pragma unroll
+      for (int k = 0; k < W; k++) v[i] += slot[i * W + k];
+    }
+  }
+}
+
+// a * b, rounded: never fused into an addition that uses it. A row's mean has
+// to be one number for all of its columns.
+__device__ __forceinline__ float mul_rounded(float a, float b) {
+#pragma clang fp contract(off)
+  return a * b;
+}
+
+// Threads of a workgroup whose rows have LPR threads each: several rows of one
+// wave or less, or one row.
+constexpr int row_threads(int lpr) { return lpr > 64 ? lpr : 256; }
+
+// The row a thread works on, of those that start at `first`: one register for
+// the wave where all of its lanes share the row, so that the row's addresses
+// are scalar.
+template <int LPR>
+__device__ __forceinline__ int64_t row_of(int64_t first) {
+  const int group = threadIdx.x / LPR;
+  if constexpr (LPR >= 64) return first + __builtin_amdgcn_readfirstlane(group);
+  return first + group;
+}
+
+// The threads that share a row (LPR) and the vectors of VEC columns each of
+// them holds (VPT), for a width: f(VEC, LPR, VPT) as integral constants. WIDE
+// is 4 where a call has an fp32 array (16 bytes of it per lane, consecutive
+// lanes side by side), else 8; rows narrower than that take a lane per column.
+template <int WIDE, class F>
+hipError_t with_row_shape(int cols, F f) {
+#define ROW_SHAPE(vec, lpr, vpt)                                                             \
+  if (cols <= lpr * vpt * vec)                                                               \
+  return f(std::integral_constant<int, vec>{}, std::integral_constant<int, lpr>{}, \
+           std::integral_constant<int, vpt>{})
+  if (cols < WIDE) ROW_SHAPE(1, 8, 1);
+  ROW_SHAPE(WIDE, 8, 1);
+  ROW_SHAPE(WIDE, 32, 1);
+  if constexpr (WIDE == 8) {
+    ROW_SHAPE(8, 32, 2);
+    ROW_SHAPE(8, 32, 3);
+    ROW_SHAPE(8, 64, 2);
+    ROW_SHAPE(8, 128, 2);
+    ROW_SHAPE(8, 256, 2);
+    ROW_SHAPE(8, 256, 3);
+    ROW_SHAPE(8, 512, 2);
+    ROW_SHAPE(8, 1024, 2);
+  } else {
+    ROW_SHAPE(4, 64, 1);
+    ROW_SHAPE(4, 64, 2);
+    ROW_SHAPE(4, 64, 3);
+    ROW_SHAPE(4, 64, 4);
+    ROW_SHAPE(4, 128, 4);
+    ROW_SHAPE(4, 256, 3);
+    ROW_SHAPE(4, 256, 4);
+    ROW_SHAPE(4, 512, 3);
+    ROW_SHAPE(4, 512, 4);
+    ROW_SHAPE(4, 1024, 4);
+  }
+#undef ROW_SHAPE
+  return hipErrorInvalidValue;
+}
+
+// Columns of a vector for a call with arrays of these types.
+template <class... T>
+constexpr int vec_of = (... || (sizeof(T) == 4)) ? 4 : 8;
 
 #endif

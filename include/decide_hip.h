@@ -460,7 +460,7 @@ int dn_set_adam_step(dn_ctx *ctx, int step);
  * their gradients and row statistics are fp32. An output may be an input's
  * very array (the same address, stride and element size); any other overlap
  * with an output is refused (DN_INVALID_ARG), as are NULL, misaligned or
- * too-narrow arrays. rows may be 0. Norms take 1 to 32,768 columns
+ * too-narrow arrays. rows may be 0. Norms take 1 to 16,384 columns
  * (DN_UNSUPPORTED beyond). No counterpart in the reference, whose model has no
  * dropout and whose LayerNorm (internal/nn/ops.go:63-138) runs inside it. */
 
@@ -498,7 +498,7 @@ int dn_layer_norm_backward_device(dn_ctx *ctx, int dy_type, int x_type, int64_t 
  * that must not share a mask need offsets (or seeds) of their own. The
  * gradient of x is dn_dropout_device of the gradient of y with the same p,
  * seed and offset. x and y are of one type or one of them is fp32; at most
- * 2^34 columns. */
+ * 2^34 - 8 columns. */
 int dn_dropout_device(dn_ctx *ctx, int x_type, int y_type, int64_t rows, int64_t cols, const void *d_x, int64_t ldx,
                       const void *d_res, int64_t ldres, float p, uint64_t seed, uint64_t offset, void *d_y,
                       int64_t ldy);
