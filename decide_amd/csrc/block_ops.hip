@@ -6,43 +6,42 @@
 
 namespace {
 
-#ifndef DROP_GRID
-#define DROP_GRID 2048
-#endif
 constexpr int kThreads = 256;
 // Most workgroups of a launch (fewer than 2^32 threads); more rows take several.
 constexpr int kGrid = 1 << 20;
 
-// LayerNorm of rows held in registers: LPR threads per row, VPT vectors of VEC
-// columns each. BOUNDARY: the row is res + dropout(x), stored to h.
-template <class X, class S, class Y, bool BOUNDARY, int VEC, int LPR, int VPT>
-__global__ __launch_bounds__(row_threads(LPR)) void norm_kernel(NormArgs a, int64_t first) {
-  constexpr int GROUPS = row_threads(LPR) / LPR, W = LPR > 64 ? LPR / 64 : 1;
-  __shared__ float slots[3 * W];
-  const int lane = threadIdx.x % LPR, cols = a.cols;
+// LayerNorm of rows held in registers. BOUNDARY: the row is res + dropout(x),
+// stored to h.
+template <class X, class S, class Y, bool BOUNDARY, class Shape>
+__global__ __launch_bounds__(Shape::MAXT) void norm_kernel(NormArgs a, int64_t first) {
+  constexpr int VEC = Shape::VEC, LPR = Shape::LPR, VPT = Shape::VPT;
+  constexpr bool WAVES = LPR == 0;
+  __shared__ float slots[WAVES ? 48 : 1];
+  const int lpr = WAVES ? blockDim.x : LPR, lane = WAVES ? threadIdx.x : threadIdx.x % lpr, cols = a.cols;
   const float inv = 1.0f / (float)cols;
-  const int64_t row = row_of<LPR>(first + (int64_t)blockIdx.x * GROUPS);
-  if (row >= a.rows) return;  // whole groups; a row of several waves has its workgroup to itself
+  const int64_t row = row_of<LPR>(first + (int64_t)blockIdx.x * Shape::ROWS);
+  if (row >= a.rows) return;  // all threads of the row
   Raw<X, VEC> x[VPT];
   Raw<S, VEC> res[BOUNDARY ? VPT : 1];
 #pragma unroll
   for (int j = 0; j < VPT; j++) {
-    const int c = VEC * (lane + j * LPR);
+    const int c = VEC * (lane + j * lpr);
     x[j] = fetch<X, VEC>((const X *)a.x + row * a.ldx, c, cols);
     if constexpr (BOUNDARY) res[j] = fetch<S, VEC>((const S *)a.res + row * a.ldres, c, cols);
   }
   float v[VPT][VEC];
 #pragma unroll
-  for (int j = 0; j < VPT; j++) unpack<X, VEC>(x[j], cols - VEC * (lane + j * LPR), v[j]);
+  for (int j = 0; j < VPT; j++) unpack<X, VEC>(x[j], cols - VEC * (lane + j * lpr), v[j]);
   if constexpr (BOUNDARY) {
-    Columns<LPR, VPT, VEC>::drop(a.mask, (uint32_t)row, lane, cols, v);
+    Columns<WAVES, VPT, VEC>::drop(a.mask, (uint32_t)row, lane, lpr, cols, v);
 #pragma unroll
     for (int j = 0; j < VPT; j++) {
-      const int c = VEC * (lane + j * LPR);
+      const int c = VEC * (lane + j * lpr);
+      if (WAVES && j > 0 && c >= cols) break;  // waves past the row; within a wave the branch costs more
       float r[VEC];
       unpack<S, VEC>(res[j], cols - c, r);
 #pragma unroll
-      for (int i = 0; i < VEC; i++) v[j][i] = (float)to_elem<S>(r[i] + v[j][i]);
+      for (int i = 0; i < VEC; i++) v[j][i] = (float)to_elem<S>(fmaf(v[j][i], a.mask.scale, r[i]));
       store<S, VEC>((S *)a.h + row * a.ldh, c, cols, v[j]);
     }
   }
@@ -58,7 +57,7 @@ __global__ __launch_bounds__(row_threads(LPR)) void norm_kernel(NormArgs a, int6
   float q[2] = {0.0f, 0.0f};
 #pragma unroll
   for (int j = 0; j < VPT; j++) {
-    const int n = cols - VEC * (lane + j * LPR);
+    const int n = cols - VEC * (lane + j * lpr);
 #pragma unroll
     for (int i = 0; i < VEC; i++) v[j][i] -= mean;
     if (n < VEC)
@@ -70,7 +69,7 @@ __global__ __launch_bounds__(row_threads(LPR)) void norm_kernel(NormArgs a, int6
       q[1] += v[j][i] * v[j][i];
     }
   }
-  row_sum<LPR>(q, slots + W);
+  row_sum<LPR>(q, slots + (WAVES ? 16 : 0));
   const float rest = mul_rounded(q[0], inv);
   const float var = q[1] * inv - rest * rest;  // a NaN stays one
   const float rstd = 1.0f / sqrtf((var < 0.0f ? 0.0f : var) + a.eps);
@@ -80,110 +79,140 @@ __global__ __launch_bounds__(row_threads(LPR)) void norm_kernel(NormArgs a, int6
   }
 #pragma unroll
   for (int j = 0; j < VPT; j++) {
-    const int c = VEC * (lane + j * LPR);
+    const int c = VEC * (lane + j * lpr);
+    if (WAVES && j > 0 && c >= cols) break;
     float w[VEC], b[VEC];
 #pragma unroll
     for (int i = 0; i < VEC; i++) w[i] = 1.0f, b[i] = 0.0f;
     if (a.w) load<float, VEC>(a.w, c, cols, w);
     if (a.b) load<float, VEC>(a.b, c, cols, b);
+    // rest is within the mean's rounding, so that its product may be rounded.
 #pragma unroll
-    for (int i = 0; i < VEC; i++) v[j][i] = (v[j][i] - rest) * rstd * w[i] + b[i];
+    for (int i = 0; i < VEC; i++) v[j][i] = fmaf(fmaf(v[j][i], rstd, -rest * rstd), w[i], b[i]);
     store<Y, VEC>((Y *)a.y + row * a.ldy, c, cols, v[j]);
   }
 }
 
-// How the threads of the elementwise kernel walk over the blocks of eight
-// columns: `per_row` blocks a row, the last of `tail` columns; from one of its
-// blocks to its next a thread goes `rows` rows and `blocks` blocks on, and one
-// row more where that passes the row's end.
-struct Walk {
-  uint32_t per_row, tail, rows, blocks;
-};
-
-// Elementwise: thread i takes blocks i, i + threads, ..., DEPTH of them loaded
-// before the first is computed; rows, blocks and offsets are carried along
-// (no product or division in the loop). NARROW: rows of less than eight
-// columns, element by element.
+// Elementwise, two vectors of VEC columns per thread: the launch's vectors i and
+// i + 64 of 128 that a wave takes, so that a wave's accesses are side by side. A
+// row has `per_row` generator blocks of eight columns, the last of `tail`; the
+// launch starts at block k0 of row r0. With VEC 4 (fp32 arrays) the two lanes
+// of a block share the generator's work as Columns::drop says. NARROW: rows of
+// less than eight columns, element by element.
 template <class X, class Y, bool RES, bool NARROW>
-__global__ __launch_bounds__(kThreads) void dropout_kernel(DropArgs a, Walk w) {
-  constexpr int DEPTH = 2;
-  const uint32_t first = blockIdx.x * kThreads + threadIdx.x, rows = (uint32_t)a.rows;
-  uint32_t row = first / w.per_row, k = first - row * w.per_row;
-  struct At {
-    int64_t x, res, y;
-  };
-  auto along = [&](int64_t r, int64_t b) { return At{r * a.ldx + 8 * b, r * a.ldres + 8 * b, r * a.ldy + 8 * b}; };
-  auto plus = [](At p, At q) { return At{p.x + q.x, RES ? p.res + q.res : 0, p.y + q.y}; };
-  const At step = along(w.rows, w.blocks), wrap = along(1, -(int64_t)w.per_row);
-  At at = along(row, k);
-  auto read = [&](auto base, int64_t off, int n) {
-    using T = std::remove_const_t<std::remove_pointer_t<decltype(base)>>;
-    Raw<T, 8> q;
-    if constexpr (NARROW) {
-      T t[8];
+__global__ __launch_bounds__(kThreads) void dropout_kernel(DropArgs a, uint32_t r0, uint32_t k0, uint32_t per_row,
+                                                           uint32_t tail) {
+  constexpr int VEC = NARROW ? 8 : vec_of<X, Y>, VPT = VEC == 4 ? 2 : 1;
+  uint32_t row[VPT], k[VPT];
+  int n[VPT], half[VPT];
+  int64_t col[VPT];
+  Raw<X, VEC> x[VPT];
+  Raw<Y, VEC> res[VPT];
 #pragma unroll
-      for (int j = 0; j < 8; j++) t[j] = base[off + min(j, n - 1)];
-      __builtin_memcpy(&q, t, sizeof(q));
-    } else {  // a partial last block as the eight elements that end with the row
-      __builtin_memcpy(&q, base + off - (8 - n), sizeof(q));
-    }
-    return q;
-  };
-  while (row < rows) {
-    Raw<X, 8> x[DEPTH];
-    Raw<Y, 8> res[RES ? DEPTH : 1];
-    uint32_t r[DEPTH], block[DEPTH];
-    At to[DEPTH];
+  for (int j = 0; j < VPT; j++) {
+    const uint32_t wave = (blockIdx.x * kThreads + threadIdx.x) & ~63u, lane = threadIdx.x & 63;
+    const uint32_t vector = wave * VPT + lane + 64 * j;       // fewer than 2^30
+    const uint32_t i = k0 + (VEC == 4 ? vector / 2 : vector);  // k0 < per_row < 2^31
+    const uint32_t down = i / per_row;
+    row[j] = r0 + down;
+    k[j] = i - down * per_row;
+    half[j] = VEC == 4 ? vector & 1 : 0;
+    const int left = k[j] == per_row - 1 ? (int)tail - 4 * half[j] : VEC;
+    n[j] = row[j] < (uint32_t)a.rows ? min(left, VEC) : 0;
+    col[j] = 8 * (int64_t)k[j] + 4 * half[j];
+  }
 #pragma unroll
-    for (int d = 0; d < DEPTH; d++) {
-      r[d] = row;
-      block[d] = k;
-      to[d] = at;
-      // Past the last row the first block is read again: no branch stands between the loads.
-      const int e = d > 0 && row >= rows ? 0 : d, n = block[e] == w.per_row - 1 ? w.tail : 8;
-      x[d] = read((const X *)a.x, to[e].x, n);
-      if constexpr (RES) res[d] = read((const Y *)a.res, to[e].res, n);
-      row += w.rows;
-      k += w.blocks;
-      at = plus(at, step);
-      if (k >= w.per_row) {
-        k -= w.per_row;
-        row++;
-        at = plus(at, wrap);
+  for (int j = 0; j < VPT; j++) {
+    auto read = [&](auto base, int64_t ld) {
+      using T = std::remove_const_t<std::remove_pointer_t<decltype(base)>>;
+      Raw<T, VEC> q;
+      if constexpr (NARROW) {
+        T t[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) t[i] = n[j] > 0 ? base[row[j] * ld + min(i, n[j] - 1)] : T(0.0f);
+        __builtin_memcpy(&q, t, sizeof(q));
+      } else {
+        // A partial vector as the VEC elements that end with the row; where there is none, the first row's first.
+        const T *p = n[j] > 0 ? base + row[j] * ld + col[j] - (VEC - n[j]) : base;
+        __builtin_memcpy(&q, p, sizeof(q));
       }
-    }
+      return q;
+    };
+    x[j] = read((const X *)a.x, a.ldx);
+    if constexpr (RES) res[j] = read((const Y *)a.res, a.ldres);
+  }
+  float v[VPT][VEC];
 #pragma unroll
-    for (int d = 0; d < DEPTH; d++) {
-      if (d > 0 && r[d] >= rows) break;
-      const int n = block[d] == w.per_row - 1 ? w.tail : 8, moved = NARROW ? 8 : n;
-      float v[1][8];
-      unpack<X, 8>(x[d], moved, v[0]);
-      Columns<1, 1, 8>::drop(a.mask, r[d], (int)block[d], 0, v);
-      if constexpr (RES) {
-        float z[8];
-        unpack<Y, 8>(res[d], moved, z);
-#pragma unroll
-        for (int j = 0; j < 8; j++) v[0][j] = z[j] + v[0][j];
-      }
-      store<Y, 8>((Y *)a.y + to[d].y, 0, n, v[0]);
+  for (int j = 0; j < VPT; j++) unpack<X, VEC>(x[j], NARROW ? VEC : n[j], v[j]);
+  if (a.mask.threshold) {
+    if constexpr (VEC == 8) {
+      const uint4 r = philox(k[0], row[0], a.mask.o0, a.mask.o1, a.mask.k0, a.mask.k1);
+      const uint32_t word[4] = {r.x, r.y, r.z, r.w};
+      drop_by<8>(a.mask, word, v[0]);
+    } else {
+      const bool odd = threadIdx.x & 1;
+      drop_pair(a.mask, odd, philox(odd ? k[VPT - 1] : k[0], odd ? row[VPT - 1] : row[0], a.mask.o0, a.mask.o1,
+                                    a.mask.k0, a.mask.k1),
+                v[0], v[VPT - 1]);
     }
+  }
+#pragma unroll
+  for (int j = 0; j < VPT; j++) {
+    if constexpr (RES) {
+      float z[VEC];
+      unpack<Y, VEC>(res[j], NARROW ? VEC : n[j], z);
+#pragma unroll
+      for (int i = 0; i < VEC; i++) v[j][i] = fmaf(v[j][i], a.mask.scale, z[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; i++) v[j][i] *= a.mask.scale;
+    }
+    store<Y, VEC>((Y *)a.y + row[j] * a.ldy + col[j], 0, n[j], v[j]);
   }
 }
 
 template <class X, class S, class Y, bool BOUNDARY>
 hipError_t norm_launch(const NormArgs &a, hipStream_t s) {
-  if (a.rows == 0) return hipSuccess;
-  return with_row_shape<vec_of<X, S, Y>>(a.cols, [&](auto vec, auto lpr, auto vpt) -> hipError_t {
-    constexpr int VEC = vec, LPR = lpr, VPT = vpt, THREADS = row_threads(LPR), GROUPS = THREADS / LPR;
-    for (int64_t first = 0; first < a.rows; first += (int64_t)kGrid * GROUPS) {
-      const int64_t groups = (std::min<int64_t>(a.rows - first, (int64_t)kGrid * GROUPS) + GROUPS - 1) / GROUPS;
-      hipLaunchKernelGGL((norm_kernel<X, S, Y, BOUNDARY, VEC, LPR, VPT>), dim3((unsigned)groups), dim3(THREADS), 0, s, a,
-                         first);
+  auto run = [&](auto shape) -> hipError_t {
+    using Shape = decltype(shape);
+    for (int64_t first = 0; first < a.rows; first += (int64_t)kGrid * Shape::ROWS) {
+      const int64_t rows = std::min<int64_t>(a.rows - first, (int64_t)kGrid * Shape::ROWS);
+      hipLaunchKernelGGL((norm_kernel<X, S, Y, BOUNDARY, Shape>), dim3((unsigned)((rows + Shape::ROWS - 1) / Shape::ROWS)),
+                         dim3(Shape::threads(a.cols)), 0, s, a, first);
       const hipError_t e = hipGetLastError();
       if (e != hipSuccess) return e;
     }
     return hipSuccess;
-  });
+  };
+  if constexpr (vec_of<X, S, Y> == 8) {
+    if (a.cols < 8) return run(RowShape<1, 8, 1>{});
+    return pick_shape<RowShape<8, 8, 1>, RowShape<8, 16, 1>, RowShape<8, 32, 1>, RowShape<8, 32, 2>, RowShape<8, 32, 3>,
+                      RowShape<8, 64, 2>, RowShape<8, 0, 2, 1024>>(a.cols, run);
+  } else {
+    if (a.cols < 4) return run(RowShape<1, 8, 1>{});
+    return pick_shape<RowShape<4, 8, 1>, RowShape<4, 16, 1>, RowShape<4, 32, 1>, RowShape<4, 64, 1>, RowShape<4, 64, 2>,
+                      RowShape<4, 64, 3>, RowShape<4, 64, 4>, RowShape<4, 0, 4, 1024>>(a.cols,
+                                                                                                              run);
+  }
+}
+
+template <class X, class Y>
+hipError_t dropout_launch(const DropArgs &a, hipStream_t s) {
+  const int64_t per_row = (a.cols + 7) / 8, total = per_row * a.rows, most = (int64_t)kGrid * kThreads;
+  for (int64_t first = 0; first < total; first += most) {
+    // A thread per block of eight columns, whether as one vector or as halves of two.
+    const int64_t blocks = std::min<int64_t>(total - first, most), groups = (blocks + kThreads - 1) / kThreads;
+    auto run = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(kThreads), 0, s, a, (uint32_t)(first / per_row),
+                         (uint32_t)(first % per_row), (uint32_t)per_row, (uint32_t)(a.cols - 8 * (per_row - 1)));
+      return hipGetLastError();
+    };
+    const hipError_t e = a.cols < 8
+                             ? (a.res ? run(dropout_kernel<X, Y, true, true>) : run(dropout_kernel<X, Y, false, true>))
+                             : (a.res ? run(dropout_kernel<X, Y, true, false>) : run(dropout_kernel<X, Y, false, false>));
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 template <class T>
@@ -199,22 +228,6 @@ hipError_t boundary_pick(int x_type, int stream_type, int y_type, const NormArgs
   if (stream_type != PREC_F32) return norm_launch<T, T, T, true>(a, s);
   if (y_type == PREC_F32) return norm_launch<float, float, float, true>(a, s);
   return x_type == PREC_F32 ? norm_launch<float, float, T, true>(a, s) : norm_launch<T, float, T, true>(a, s);
-}
-
-template <class X, class Y>
-hipError_t dropout_launch(const DropArgs &a, hipStream_t s) {
-  const int64_t per_row = (a.cols + 7) / 8, total = per_row * a.rows;
-  if (total == 0) return hipSuccess;
-  // Enough threads to fill the CUs; more blocks are more rounds of the loop.
-  const int64_t grid = std::min<int64_t>((total + kThreads - 1) / kThreads, DROP_GRID), threads = grid * kThreads;
-  const Walk w{(uint32_t)per_row, (uint32_t)(a.cols - 8 * (per_row - 1)), (uint32_t)(threads / per_row),
-               (uint32_t)(threads % per_row)};
-  auto run = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(kThreads), 0, s, a, w);
-    return hipGetLastError();
-  };
-  if (a.cols < 8) return a.res ? run(dropout_kernel<X, Y, true, true>) : run(dropout_kernel<X, Y, false, true>);
-  return a.res ? run(dropout_kernel<X, Y, true, false>) : run(dropout_kernel<X, Y, false, false>);
 }
 
 template <class T>

@@ -38,42 +38,60 @@ __device__ __forceinline__ uint4 philox(uint32_t c0, uint32_t c1, uint32_t c2, u
   return make_uint4(c0, c1, c2, c3);
 }
 
-// Drops elements in place, from the generator's words that hold their 16-bit
+// Drops elements in place (the scale of the others is the caller's, one
+// multiply-add with what they are added to), from the generator's words that hold their 16-bit
 // draws: element j takes half j % 2 (0 low) of word j / 2. A dropped element
 // is 0 whatever it was (also an infinity or a NaN), so it is selected, not
 // multiplied. A half is at least the threshold t > 0 where its word, with that
 // half in the upper bits, is above 65536 t - 1: the lower bits only add, and
 // at t = 65536 nothing is above 2^32 - 1.
-__device__ __forceinline__ float keep_scaled(const DropMask &m, uint32_t upper, float v) {
-  return upper > (m.threshold << 16) - 1u ? v * m.scale : 0.0f;
+__device__ __forceinline__ float keep(const DropMask &m, uint32_t upper, float v) {
+  return upper > (m.threshold << 16) - 1u ? v : 0.0f;
 }
 template <int N>
 __device__ __forceinline__ void drop_by(const DropMask &m, const uint32_t (&word)[N / 2], float (&v)[N]) {
 #pragma unroll
   for (int j = 0; j < N / 2; j++) {
-    v[2 * j] = keep_scaled(m, word[j] << 16, v[2 * j]);
-    v[2 * j + 1] = keep_scaled(m, word[j], v[2 * j + 1]);
+    v[2 * j] = keep(m, word[j] << 16, v[2 * j]);
+    v[2 * j + 1] = keep(m, word[j], v[2 * j + 1]);
   }
 }
 
-// The columns of a row that one of its LPR threads holds: VPT vectors of VEC,
-// vector j at column VEC * (lane + j * LPR).
-template <int LPR, int VPT, int VEC>
+// Two vectors of four columns, halves of two generator blocks that the lane and
+// its neighbour share: of the first vectors' block r is in the even lane, of
+// the second ones' in the odd lane, and each hands the other its half (the even
+// lane holds the lower four columns of both). Both lanes take part.
+__device__ __forceinline__ void drop_pair(const DropMask &m, bool odd, const uint4 &r, float (&first)[4],
+                                          float (&second)[4]) {
+  const uint32_t low[2] = {r.x, r.y}, high[2] = {r.z, r.w};
+  uint32_t a[2], b[2];
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    const uint32_t mine = odd ? high[i] : low[i];
+    const uint32_t other = dpp_u32<0xB1>(odd ? low[i] : high[i]);  // the neighbour's: quad_perm 1,0,3,2
+    a[i] = odd ? other : mine;
+    b[i] = odd ? mine : other;
+  }
+  drop_by<4>(m, a, first);
+  drop_by<4>(m, b, second);
+}
+
+// The columns of a row that one of its `lpr` threads holds: VPT vectors of VEC,
+// vector j at column VEC * (lane + j * lpr). WAVES: the row has several waves.
+template <bool WAVES, int VPT, int VEC>
 struct Columns {
   // The elements of a row of `cols` dropped in place. One generator block covers
   // eight columns: a vector of eight, or the vectors of four of two neighbouring
-  // lanes, or a row of less than eight columns with one lane each. The two
-  // lanes share the work: of vectors j and j + 1 the even lane generates j's
-  // block and the odd one j + 1's, and each hands the other its half. They skip
-  // a vector together, when the even lane's starts past the row.
-  static __device__ __forceinline__ void drop(const DropMask &m, uint32_t row, int lane, int cols,
+  // lanes (drop_pair), or a row of less than eight columns with one lane each.
+  // Waves that lie past the row skip a vector, both lanes of a pair or neither.
+  static __device__ __forceinline__ void drop(const DropMask &m, uint32_t row, int lane, int lpr, int cols,
                                               float (&v)[VPT][VEC]) {
     if (m.threshold == 0) return;
     if constexpr (VEC == 8) {
 #pragma unroll
       for (int j = 0; j < VPT; j++) {
-        const int block = lane + j * LPR;
-        if (j > 0 && 8 * block >= cols) break;
+        const int block = lane + j * lpr;
+        if (WAVES && j > 0 && 8 * block >= cols) break;
         const uint4 r = philox((uint32_t)block, row, m.o0, m.o1, m.k0, m.k1);
         const uint32_t word[4] = {r.x, r.y, r.z, r.w};
         drop_by<8>(m, word, v[j]);
@@ -81,32 +99,19 @@ struct Columns {
     } else if constexpr (VEC == 1) {
       const uint4 r = philox(0, row, m.o0, m.o1, m.k0, m.k1);
       const uint32_t word = lane < 4 ? (lane < 2 ? r.x : r.y) : (lane < 6 ? r.z : r.w);
-      v[0][0] = keep_scaled(m, lane & 1 ? word : word << 16, v[0][0]);
+      v[0][0] = keep(m, lane & 1 ? word : word << 16, v[0][0]);
     } else {
       const bool odd = lane & 1;
 #pragma unroll
       for (int j = 0; j < VPT; j += 2) {
         const bool pair = j + 1 < VPT;
-        if (j > 0 && 4 * ((lane & ~1) + j * LPR) >= cols) break;
-        const uint4 r = philox((uint32_t)(lane + (j + (pair && odd ? 1 : 0)) * LPR) >> 1, row, m.o0, m.o1, m.k0, m.k1);
-        const uint32_t low[2] = {r.x, r.y}, high[2] = {r.z, r.w};
-        uint32_t mine[2], other[2];
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-          mine[i] = odd ? high[i] : low[i];
-          if (pair) other[i] = dpp_u32<0xB1>(odd ? low[i] : high[i]);  // the neighbour's: quad_perm 1,0,3,2
-        }
+        if (WAVES && j > 0 && 4 * ((lane & ~1) + j * lpr) >= cols) break;
+        const uint4 r = philox((uint32_t)(lane + (j + (pair && odd ? 1 : 0)) * lpr) >> 1, row, m.o0, m.o1, m.k0, m.k1);
         if (pair) {
-          uint32_t first[2], second[2];
-#pragma unroll
-          for (int i = 0; i < 2; i++) {
-            first[i] = odd ? other[i] : mine[i];
-            second[i] = odd ? mine[i] : other[i];
-          }
-          drop_by<4>(m, first, v[j]);
-          drop_by<4>(m, second, v[j + 1 < VPT ? j + 1 : j]);
+          drop_pair(m, odd, r, v[j], v[j + 1 < VPT ? j + 1 : j]);
         } else {
-          drop_by<4>(m, mine, v[j]);
+          const uint32_t word[2] = {odd ? r.z : r.x, odd ? r.w : r.y};
+          drop_by<4>(m, word, v[j]);
         }
       }
     }
@@ -175,46 +180,47 @@ __device__ __forceinline__ void store(T *row, int c, int cols, const float (&v)[
   }
 }
 
-// The sum of each v[i] over the LPR consecutive threads that share a row, in
-// all of them: DPP moves within 16 lanes and row swaps across them (no LDS
-// round trips: 10 dependent steps of ~8 cycles where a shuffle takes ~60), and
-// for a row over several waves one exchange through LDS. The order of the sum
-// depends on LPR alone. `slot`: LDS that no other reduction of the same loop
-// iteration uses, so that one barrier per reduction is enough.
+// The sum of each v[i] over the threads that share a row, in all of them: LPR
+// consecutive threads, or (0) the workgroup. DPP moves within 16 lanes and row
+// swaps across them (no LDS round trips: steps of ~8 cycles where a shuffle
+// takes ~60), and for a workgroup one exchange of its waves' sums (at most 16)
+// through LDS. The order of the sum depends on the number of threads alone.
+// `slot`: N * 16 floats of LDS that no other reduction of the same row uses, so
+// that one barrier per reduction is enough.
 template <int LPR, int N>
 __device__ __forceinline__ void row_sum(float (&v)[N], float *slot) {
   auto add = [&](auto move) {
 #pragma unroll
     for (int i = 0; i < N; i++) v[i] += __uint_as_float(move(__float_as_uint(v[i])));
   };
-  add([](unsigned x) { return dpp_u32<0xB1>(x); });  // quad_perm 1,0,3,2
-  add([](unsigned x) { return dpp_u32<0x4E>(x); });  // quad_perm 2,3,0,1
-  add([](unsigned x) { return dpp_u32<0x141>(x); });  // row_half_mirror
-  if constexpr (LPR >= 16) add([](unsigned x) { return dpp_u32<0x140>(x); });  // row_mirror
-  if constexpr (LPR >= 32)
+  auto add16 = [&] {
+    add([](unsigned x) { return dpp_u32<0xB1>(x); });   // quad_perm 1,0,3,2
+    add([](unsigned x) { return dpp_u32<0x4E>(x); });   // quad_perm 2,3,0,1
+    add([](unsigned x) { return dpp_u32<0x141>(x); });  // row_half_mirror
+    if constexpr (LPR != 8) add([](unsigned x) { return dpp_u32<0x140>(x); });  // row_mirror
+  };
+  add16();
+  if constexpr (LPR == 0 || LPR >= 32)
 #pragma unroll
     for (int i = 0; i < N; i++) {
       const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v[i]), __float_as_uint(v[i]), false, false);
       v[i] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
     }
-  if constexpr (LPR >= 64)
+  if constexpr (LPR == 0 || LPR >= 64)
 #pragma unroll
     for (int i = 0; i < N; i++) {
       const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[i]), __float_as_uint(v[i]), false, false);
       v[i] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
     }
-  if constexpr (LPR > 64) {
-    constexpr int W = LPR / 64;
+  if constexpr (LPR == 0) {
     if ((threadIdx.x & 63) == 0)
 #pragma unroll
-      for (int i = 0; i < N; i++) slot[i * W + (threadIdx.x >> 6)] = v[i];
+      for (int i = 0; i < N; i++) slot[16 * i + (threadIdx.x >> 6)] = v[i];
     __syncthreads();
+    const int k = threadIdx.x & 15;
 #pragma unroll
-    for (int i = 0; i < N; i++) {
-      v[i] = 0;
-#pragma unroll
-      for (int k = 0; k < W; k++) v[i] += slot[i * W + k];
-    }
+    for (int i = 0; i < N; i++) v[i] = k < (int)(blockDim.x >> 6) ? slot[16 * i + k] : 0.0f;
+    add16();
   }
 }
 
@@ -225,59 +231,44 @@ __device__ __forceinline__ float mul_rounded(float a, float b) {
   return a * b;
 }
 
-// Threads of a workgroup whose rows have LPR threads each: several rows of one
-// wave or less, or one row.
-constexpr int row_threads(int lpr) { return lpr > 64 ? lpr : 256; }
+// Threads of a workgroup whose rows have LPR threads each.
+constexpr int kRowThreads = 256;
 
-// The row a thread works on, of those that start at `first`: one register for
-// the wave where all of its lanes share the row, so that the row's addresses
-// are scalar.
+// The row a thread works on, of those that start at `first`: LPR threads per
+// row, or (0) the workgroup. One register for the wave where all of its lanes
+// share the row, so that the row's addresses are scalar.
 template <int LPR>
 __device__ __forceinline__ int64_t row_of(int64_t first) {
-  const int group = threadIdx.x / LPR;
-  if constexpr (LPR >= 64) return first + __builtin_amdgcn_readfirstlane(group);
+  if constexpr (LPR == 0) return first;
+  const int group = threadIdx.x / (LPR ? LPR : 1);
+  if constexpr (LPR == 64) return first + __builtin_amdgcn_readfirstlane(group);
   return first + group;
 }
 
-// The threads that share a row (LPR) and the vectors of VEC columns each of
-// them holds (VPT), for a width: f(VEC, LPR, VPT) as integral constants. WIDE
-// is 4 where a call has an fp32 array (16 bytes of it per lane, consecutive
-// lanes side by side), else 8; rows narrower than that take a lane per column.
-template <int WIDE, class F>
-hipError_t with_row_shape(int cols, F f) {
-#define ROW_SHAPE(vec, lpr, vpt)                                                             \
-  if (cols <= lpr * vpt * vec)                                                               \
-  return f(std::integral_constant<int, vec>{}, std::integral_constant<int, lpr>{}, \
-           std::integral_constant<int, vpt>{})
-  if (cols < WIDE) ROW_SHAPE(1, 8, 1);
-  ROW_SHAPE(WIDE, 8, 1);
-  ROW_SHAPE(WIDE, 32, 1);
-  if constexpr (WIDE == 8) {
-    ROW_SHAPE(8, 32, 2);
-    ROW_SHAPE(8, 32, 3);
-    ROW_SHAPE(8, 64, 2);
-    ROW_SHAPE(8, 128, 2);
-    ROW_SHAPE(8, 256, 2);
-    ROW_SHAPE(8, 256, 3);
-    ROW_SHAPE(8, 512, 2);
-    ROW_SHAPE(8, 1024, 2);
-  } else {
-    ROW_SHAPE(4, 64, 1);
-    ROW_SHAPE(4, 64, 2);
-    ROW_SHAPE(4, 64, 3);
-    ROW_SHAPE(4, 64, 4);
-    ROW_SHAPE(4, 128, 4);
-    ROW_SHAPE(4, 256, 3);
-    ROW_SHAPE(4, 256, 4);
-    ROW_SHAPE(4, 512, 3);
-    ROW_SHAPE(4, 512, 4);
-    ROW_SHAPE(4, 1024, 4);
+// How the threads share rows of a width: LPR threads of a workgroup of
+// kRowThreads per row, or (LPR 0) a workgroup per row of as many waves as VPT
+// vectors of VEC columns per thread need, MAXT threads at most.
+template <int VEC_, int LPR_, int VPT_, int MAXT_ = kRowThreads>
+struct RowShape {
+  static constexpr int VEC = VEC_, LPR = LPR_, VPT = VPT_, MAXT = MAXT_;
+  static constexpr int ROWS = LPR ? kRowThreads / (LPR ? LPR : 1) : 1;  // of a workgroup
+  static int threads(int cols) {
+    return LPR ? kRowThreads : ((cols + VEC * VPT - 1) / (VEC * VPT) + 63) / 64 * 64;
   }
-#undef ROW_SHAPE
+  static bool takes(int cols) { return cols <= VEC * VPT * (LPR ? LPR : MAXT); }
+};
+
+// Calls f with the first shape of the list that takes the width.
+template <class First, class... Rest, class F>
+hipError_t pick_shape(int cols, F f) {
+  if (First::takes(cols)) return f(First{});
+  if constexpr (sizeof...(Rest) > 0) return pick_shape<Rest...>(cols, f);
   return hipErrorInvalidValue;
 }
 
-// Columns of a vector for a call with arrays of these types.
+// Columns of a vector for a call with arrays of these types: 4 with an fp32
+// array (16 bytes of it per lane, consecutive lanes side by side), else 8. Rows
+// narrower than that take a lane per column.
 template <class... T>
 constexpr int vec_of = (... || (sizeof(T) == 4)) ? 4 : 8;
 
