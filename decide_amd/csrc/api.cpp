@@ -81,7 +81,8 @@ void release_train(TrainState &tr) {
   DevBuf *bufs[] = {&tr.dcur, &tr.dprev, &tr.dh1[0], &tr.dh1[1], &tr.dact, &tr.dwi[0], &tr.dwi[1], &tr.dn2,
                     &tr.dctx, &tr.dqkv[0], &tr.dqkv[1], &tr.dn1, &tr.dop_out, &tr.dop_h1, &tr.dsum, &tr.part,
                     &tr.lnpart, &tr.dE, &tr.dl, &tr.contrib, &tr.emb_order, &tr.emb_seg, &tr.emb_id, &tr.sq_part,
-                    &tr.sq_out, &tr.opT[0], &tr.opT[1], &tr.emb_mean, &tr.emb_rstd, &tr.mt};
+                    &tr.sq_out, &tr.opT[0], &tr.opT[1], &tr.emb_mean, &tr.emb_rstd, &tr.mt, &tr.sub,
+                    &tr.drop_out[0], &tr.drop_out[1], &tr.drop_h1[0], &tr.drop_h1[1], &tr.norm_work};
   if (tr.side) (void)hipStreamSynchronize(tr.side);
   for (DevBuf *b : bufs) release(*b);
   for (int i = 0; i < 2; i++) {
@@ -425,6 +426,9 @@ struct Pass {
   // Attention with the keys split over waves (attn_key_split).
   bool key_split = false;
   int rows = 0;  // the whole batch's tokens (inference)
+  // Training with dropout: its setting, and the buffer of a sub-layer's output.
+  const DropSetting *drop = nullptr;
+  float *sub = nullptr;
   Workspace w;
   const int32_t *ids, *pos, *opt;
   hipStream_t s;
@@ -485,6 +489,40 @@ hipError_t layer_gemm(const Config &g, int epi, const GemmArgs &a0, hipStream_t 
   return g.generic ? launch_gemm_generic(g.precision, epi, a, s) : launch_gemm(g.precision, epi, a, s, ln);
 }
 
+// h = res + dropout(p.sub), and y = LayerNorm(h) with the norm weight of that
+// name; site: drop_mask's.
+hipError_t add_norm(dn_ctx *c, const Pass &p, int l, int site, const float *res, float *h, const std::string &norm,
+                    void *y, float *mean, float *rstd) {
+  const Config &g = c->cfg;
+  NormArgs a{};
+  a.rows = p.w.T;
+  a.cols = g.hidden;
+  a.x = p.sub;
+  a.res = res;
+  a.h = h;
+  a.y = y;
+  a.ldx = a.ldres = a.ldh = a.ldy = g.hidden;
+  a.mask = drop_mask(*p.drop, g.layers, l, site);
+  a.w = (const float *)W(c, norm);
+  a.eps = g.eps;
+  a.mean = mean;
+  a.rstd = rstd;
+  return launch_boundary(PREC_F32, PREC_F32, g.precision, a, p.s);
+}
+
+// h = res + dropout(p.sub).
+hipError_t add_dropped(dn_ctx *c, const Pass &p, int l, int site, const float *res, float *h) {
+  DropArgs a{};
+  a.rows = p.w.T;
+  a.cols = c->cfg.hidden;
+  a.x = p.sub;
+  a.res = res;
+  a.y = h;
+  a.ldx = a.ldres = a.ldy = a.cols;
+  a.mask = drop_mask(*p.drop, c->cfg.layers, l, site);
+  return launch_dropout(PREC_F32, PREC_F32, a, p.s);
+}
+
 // The launches of encoder layer l over the pass's tokens: the residual stream
 // enters in `in`, leaves the attention half in h1 and the layer in out (the
 // same buffer unless training keeps them apart); x1 is the QKV input of layer
@@ -500,10 +538,13 @@ hipError_t layer_gemm(const Config &g, int epi, const GemmArgs &a0, hipStream_t 
 // LayerNorm (p.fold): fold_in, the previous layer's MlpWo left attn_norm's
 // operand in the workspace's xn and its statistics (this layer's QKV applies
 // the norm); mlp_norm is folded into Wo and Wi; fold_out, this layer's
-// MlpWo leaves the next layer's attn_norm operand the same way.
+// MlpWo leaves the next layer's attn_norm operand the same way. With dropout
+// (p.drop) Wo and MlpWo write their product to p.sub, and the boundary operator
+// adds it, dropped, to the residual stream and applies the norm that follows:
+// mlp_norm, or the next layer's attn_norm, whose activations go to next.
 int enqueue_layer(dn_ctx *c, const Pass &p, int l, float *in, float *h1, float *out, void *x1, LayerSave *S,
                   hipEvent_t *ev, bool attn_only = false, int in_parts = 0, int *mo_parts = nullptr,
-                  bool fold_in = false, bool fold_out = false) {
+                  bool fold_in = false, bool fold_out = false, LayerSave *next = nullptr) {
   const Config &g = c->cfg;
   const int H = g.hidden, I = g.inter, prec = g.precision;
   const Workspace &w = p.w;
@@ -522,8 +563,8 @@ int enqueue_layer(dn_ctx *c, const Pass &p, int l, float *in, float *h1, float *
   float *const mlp_part = (float *)w.qkv, *const attn_part = (float *)w.ctx;
   if (l > 0) {
     x1 = S ? S->n1.p : w.xn;
-    if (fold_in) {
-      // the previous layer's MlpWo wrote x1 and the row statistics
+    if (fold_in || p.drop) {
+      // the previous layer's MlpWo, or the boundary after it, wrote x1 and the row statistics
     } else if (in_parts > 0 && split)
       HIPCHK(c, "ln(attn_norm)", launch_ln_parts(prec, in, w.part, in_parts, T, H,
                                                  (const float *)W(c, pf + "attn_norm.weight"), g.eps, x1, s));
@@ -611,7 +652,14 @@ int enqueue_layer(dn_ctx *c, const Pass &p, int l, float *in, float *h1, float *
   // layer's attn_norm means when its QKV folded too (0 otherwise).
   float *const mlp_mprev = fold_in ? w.lmean1 : nullptr;
   const int wo_parts = split ? small_split_parts(prec, T, H, H) : 1;
-  if (wo_parts > 1) {
+  if (p.drop) {
+    o.C = p.sub;
+    o.res = nullptr;
+    o.accumulate = 0;
+    PROBED(ev, DN_PROBE_WO, "gemm(Wo)", layer_gemm(g, EPI_F32, o, s));
+    HIPCHK(c, "boundary(mlp_norm)", add_norm(c, p, l, 0, in, h1, pf + "mlp_norm.weight", x2,
+                                             S ? (float *)S->mean2.p : nullptr, S ? (float *)S->rstd2.p : nullptr));
+  } else if (wo_parts > 1) {
     o.skinny_regs = g.skinny_regs ? 1 : 0;
     PROBED(ev, DN_PROBE_WO, "gemm(Wo)", launch_gemm_small_split(prec, o, wo_parts, w.part, s));
     HIPCHK(c, "ln(mlp_norm)", launch_ln_parts(prec, h1, w.part, wo_parts, T, H,
@@ -686,7 +734,18 @@ int enqueue_layer(dn_ctx *c, const Pass &p, int l, float *in, float *h1, float *
     mf.lparts = lparts;
     mf.mprev = w.lmean2;
   }
-  if (parts > 1)
+  if (p.drop) {
+    mo.C = p.sub;
+    mo.res = nullptr;
+    mo.accumulate = 0;
+    PROBED(ev, DN_PROBE_MLPWO, "gemm(MlpWo)", layer_gemm(g, EPI_F32, mo, s));
+    if (l + 1 < g.layers)
+      HIPCHK(c, "boundary(attn_norm)",
+             add_norm(c, p, l, 1, h1, out, layer_prefix(l + 1) + "attn_norm.weight", next ? next->n1.p : w.xn,
+                      next ? (float *)next->mean1.p : nullptr, next ? (float *)next->rstd1.p : nullptr));
+    else
+      HIPCHK(c, "dropout(last)", add_dropped(c, p, l, 1, h1, out));
+  } else if (parts > 1)
     PROBED(ev, DN_PROBE_MLPWO, "gemm(MlpWo)", launch_gemm_small_split(prec, mo, parts, w.part, s));
   else
     PROBED(ev, DN_PROBE_MLPWO, "gemm(MlpWo)", layer_gemm(g, fold_out ? EPI_F32_LN : EPI_F32, mo, s, &mf));
@@ -1159,6 +1218,7 @@ int forward_core(dn_ctx *c, int nseq, const int32_t *seq_len, const int32_t *d_i
     }
     HIPCHK(c, "hipMalloc", ensure(tr.emb_mean, sizeof(float) * T));
     HIPCHK(c, "hipMalloc", ensure(tr.emb_rstd, sizeof(float) * T));
+    if (tr.drop.p > 0.0f) HIPCHK(c, "hipMalloc", ensure(tr.sub, sizeof(float) * T * H));
   }
   if (ws && (!c->rope_ready || !c->err_flag.p))
     return fail(c, DN_INVALID_ARG, "decide_hip: set-up incomplete (dn_set_config builds the RoPE tables)");
@@ -1174,6 +1234,10 @@ int forward_core(dn_ctx *c, int nseq, const int32_t *seq_len, const int32_t *d_i
   ps.opt = d_opt;
   ps.s = c->stream;
   ps.rows = train ? 0 : T;
+  if (train && tr.drop.p > 0.0f) {
+    ps.drop = &tr.drop;
+    ps.sub = (float *)tr.sub.p;
+  }
   ps.fold = !train && w.lmean1 && fold_eligible(c, T);
   ps.ln_cols = T <= kLnNarrowTokens ? kLnPartNarrow : kLnPartWide;
   // Training keeps the tile walk in bf16: its gradients cancel over a
@@ -1212,7 +1276,7 @@ int forward_core(dn_ctx *c, int nseq, const int32_t *seq_len, const int32_t *d_i
     // or the option-row layer reads it).
     int parts = 0;
     rc = enqueue_layer(c, ps, l, in, h1, out, xn0, S, ev, rows_tail && l == L - 1, pending,
-                       !train && l + 1 < nfull ? &parts : nullptr, l > 0, l + 1 < nfull);
+                       !train && l + 1 < nfull ? &parts : nullptr, l > 0, l + 1 < nfull, saved(l + 1));
     if (rc) return rc;
     pending = parts;
     cur = out;
@@ -1236,6 +1300,8 @@ int forward_core(dn_ctx *c, int nseq, const int32_t *seq_len, const int32_t *d_i
     tr.have_forward = true;
     tr.T = T;
     tr.R = R;
+    tr.used = tr.drop;
+    if (tr.drop.p > 0.0f) tr.drop.step++;
   }
   return DN_OK;
 }

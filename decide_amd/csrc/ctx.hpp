@@ -9,6 +9,7 @@
 #include <vector>
 
 #include "../../include/decide_hip.h"
+#include "block_ops.hpp"
 #include "common.hpp"
 
 struct DevBuf {
@@ -60,6 +61,13 @@ struct LayerSave {
   DevBuf mean1, rstd1, mean2, rstd2;  // fp32 [T]: attn_norm and mlp_norm row statistics
 };
 
+// Dropout of the sub-layers' outputs (dn_set_dropout): the masks of training
+// forward `step`.
+struct DropSetting {
+  float p = 0.0f;
+  uint64_t seed = 0, step = 0;
+};
+
 struct TrainState {
   bool enabled = false;
   int train_from = 0;
@@ -70,6 +78,13 @@ struct TrainState {
   int T = 0, R = 0;
   std::vector<int32_t> ids;   // token ids of the last training forward
   DevBuf emb_mean, emb_rstd;  // emb norm row statistics of the last training forward
+  // Dropout: of the next training forward, and of the last one (the backward
+  // regenerates its masks). sub: fp32 [T x H], a sub-layer's output before it
+  // is dropped; drop_out / drop_h1, by layer parity like dh1: the operand-type
+  // gradients of the MlpWo and Wo products (dropout's of dout and dh1);
+  // norm_work: the partial sums of a norm's weight gradient.
+  DropSetting drop, used;
+  DevBuf sub, drop_out[2], drop_h1[2], norm_work;
   // dh1, dwi and dqkv alternate by layer parity: the weight-gradient stream
   // transposes them while the main stream works on the next layer. dop_out /
   // dop_h1: bf16 copies of dout and dh1 (the input-gradient GEMMs' operands).
@@ -225,6 +240,8 @@ hipError_t ensure(DevBuf &b, size_t bytes);
 void release(DevBuf &b);
 void release_slot(TensorSlot &t);
 void release_train(TrainState &tr);
+// The mask of a dropout site: after layer l's attention (site 0) or MLP (1).
+DropMask drop_mask(const DropSetting &d, int layers, int l, int site);
 uint16_t f32_to_bf16_rne(float f);
 std::string layer_prefix(int l);
 const void *W(dn_ctx *c, const std::string &name);

@@ -13,6 +13,9 @@
 //   dqkv = attention backward (RoPE inverse on dq, dk)
 //   gWqkv += dqkv^T . n1           dn1 = dqkv . Wqkv
 //   dprev = dh1 + LNbwd(dn1)       (attn_norm; layer 0: dh1 + dn1)
+// With dropout (dn_set_dropout) the products' gradients are dropout's of dout
+// (MlpWo) and of dh1 (Wo), from the regenerated masks, written in the operand
+// type beside dprev and dh1 by the boundary operator's backward pass.
 // Input-gradient GEMMs run on the forward GEMM kernel with a transposed copy
 // of the weights; weight-gradient GEMMs (a reduction over tokens) run on
 // transposed operand copies, with partial products of token ranges summed in
@@ -27,9 +30,16 @@
 #include <string>
 #include <vector>
 
+#include "block_check.hpp"
 #include "ctx.hpp"
 
 using namespace dnh;
+
+DropMask dnh::drop_mask(const DropSetting &d, int layers, int l, int site) {
+  DropMask m{};
+  (void)blockchk::mask("dropout", d.p, d.seed, d.step * (2 * (uint64_t)layers) + 2 * l + site, &m);
+  return m;
+}
 
 namespace {
 
@@ -229,6 +239,14 @@ int backward_impl(dn_ctx *c, const float *dlogits) {
   HIPCHK(c, "hipMalloc", ensure(tr.dctx, es * TH));
   HIPCHK(c, "hipMalloc", ensure(tr.dop_out, es * TH));
   HIPCHK(c, "hipMalloc", ensure(tr.dop_h1, es * TH));
+  const bool drop = tr.used.p > 0.0f;
+  if (drop) {
+    for (int q = 0; q < 2; q++) {
+      HIPCHK(c, "hipMalloc", ensure(tr.drop_out[q], es * TH));
+      HIPCHK(c, "hipMalloc", ensure(tr.drop_h1[q], es * TH));
+    }
+    HIPCHK(c, "hipMalloc", ensure(tr.norm_work, sizeof(float) * (size_t)norm_grad_work(T, H)));
+  }
   // Transposed operands of one layer's weight-gradient GEMMs: dout, act, dwi,
   // n2, dh1, ctx, dqkv, n1 (rows of Tp tokens), one arena per layer parity.
   const size_t opT_rows = (size_t)8 * H + 3 * I;
@@ -286,6 +304,28 @@ int backward_impl(dn_ctx *c, const float *dlogits) {
   const bool bf = prec == DN_PRECISION_BF16;
   const bool fuse_geglu = gemm_epi_ok(prec, EPI_GEGLU_BWD, T);
   float *lnpart = (float *)tr.lnpart.p;
+  // dres = dh + the gradient of dy through the norm of h, dx = dropout's of it
+  // in the operand type; the norm's weight gradient is added up.
+  auto boundary = [&](const float *dy, const float *dh, const DevBuf &h, const std::string &norm, const DevBuf &mean,
+                      const DevBuf &rstd, const DropMask &mask, float *dres, void *dx) {
+    NormGradArgs a{};
+    a.rows = T;
+    a.cols = H;
+    a.dy = dy;
+    a.dh = dh;
+    a.h = h.p;
+    a.lddy = a.lddh = a.ldh = a.lddres = a.lddx = H;
+    a.w = (const float *)W(c, norm);
+    a.mean = (const float *)mean.p;
+    a.rstd = (const float *)rstd.p;
+    a.mask = mask;
+    a.dres = dres;
+    a.dx = dx;
+    a.dw = grad(norm);
+    a.accumulate = 1;
+    a.work = (float *)tr.norm_work.p;
+    return launch_boundary_grad(PREC_F32, PREC_F32, prec, a, s);
+  };
   for (int l = L - 1; l >= tr.train_from && l >= 0; l--) {
     const std::string p = layer_prefix(l);
     const LayerSave &S = tr.layers[l];
@@ -317,8 +357,19 @@ int backward_impl(dn_ctx *c, const float *dlogits) {
     // layer above's LN backward (for the top layer, by this transpose, which
     // also gives its transposed copy; lower layers' transposes run on the
     // weight-gradient stream).
-    if (top) RC(b.transpose(0, dcur, H, doutT, bf ? tr.dop_out.p : nullptr));
-    const void *dout_op = bf ? tr.dop_out.p : (const void *)dcur;
+    if (top && drop) {
+      DropArgs da{};
+      da.rows = T;
+      da.cols = da.ldx = da.ldy = H;
+      da.x = dcur;
+      da.y = tr.drop_out[par].p;
+      da.mask = drop_mask(tr.used, L, l, 1);
+      HIPCHK(c, "dropout(dout)", launch_dropout(PREC_F32, prec, da, s));
+      RC(b.transpose(prec, tr.drop_out[par].p, H, doutT));
+    } else if (top) {
+      RC(b.transpose(0, dcur, H, doutT, bf ? tr.dop_out.p : nullptr));
+    }
+    const void *dout_op = drop ? tr.drop_out[par].p : bf ? tr.dop_out.p : (const void *)dcur;
 
     // MLP: out = h1 + MlpWo(act)
     if (fuse_geglu) {  // dwi straight from the GEMM's epilogue
@@ -341,13 +392,17 @@ int backward_impl(dn_ctx *c, const float *dlogits) {
     }
     RC(b.gemm(EPI_F32, T, H, 2 * I, dwi, 2 * I, wt(p + "mlp.Wi.weight"), 2 * I, dn2, H));
     float *lnp_mlp = lnpart + (size_t)(2 * par) * lnslot, *lnp_attn = lnp_mlp + lnslot;
-    HIPCHK(c, "ln_bwd(mlp_norm)", launch_ln_bwd(dh1, dcur, dn2, (const float *)S.h1.p, nullptr,
+    if (drop)
+      HIPCHK(c, "boundary_bwd(mlp_norm)", boundary(dn2, dcur, S.h1, p + "mlp_norm.weight", S.mean2, S.rstd2,
+                                                   drop_mask(tr.used, L, l, 0), dh1, tr.drop_h1[par].p));
+    else
+      HIPCHK(c, "ln_bwd(mlp_norm)", launch_ln_bwd(dh1, dcur, dn2, (const float *)S.h1.p, nullptr,
                                                 (const float *)S.mean2.p, (const float *)S.rstd2.p,
                                                 (const float *)W(c, p + "mlp_norm.weight"), g.eps, T, H, lnp_mlp,
                                                 nullptr, s, bf ? tr.dop_h1.p : nullptr));
 
     // Attention: h1 = in + Wo(ctx)
-    const void *dh1_op = bf ? tr.dop_h1.p : (const void *)dh1;
+    const void *dh1_op = drop ? tr.drop_h1[par].p : bf ? tr.dop_h1.p : (const void *)dh1;
     RC(b.gemm(EPI_STORE, T, H, H, dh1_op, H, wt(p + "attn.Wo.weight"), H, tr.dctx.p, H));
 
     AttnBwdArgs at{};
@@ -383,7 +438,10 @@ int backward_impl(dn_ctx *c, const float *dlogits) {
     RC(mark(DN_PROBE_BWD_DGRAD_QKV, 1, s));
     // dprev held the layer above's dout: its transpose must be done.
     HIPCHK(c, "hipStreamWaitEvent", hipStreamWaitEvent(s, tr.ev_trans[par ^ 1], 0));
-    if (l > 0) {
+    if (l > 0 && drop) {
+      HIPCHK(c, "boundary_bwd(attn_norm)", boundary(dn1, dh1, S.hs, p + "attn_norm.weight", S.mean1, S.rstd1,
+                                                    drop_mask(tr.used, L, l - 1, 1), dprev, tr.drop_out[par ^ 1].p));
+    } else if (l > 0) {
       HIPCHK(c, "ln_bwd(attn_norm)", launch_ln_bwd(dprev, dh1, dn1, (const float *)S.hs.p, nullptr,
                                                    (const float *)S.mean1.p, (const float *)S.rstd1.p,
                                                    (const float *)W(c, p + "attn_norm.weight"), g.eps, T, H, lnp_attn,
@@ -399,12 +457,13 @@ int backward_impl(dn_ctx *c, const float *dlogits) {
     // The gradients' transposes and the LayerNorm weight gradients (their
     // buffers alternate by layer parity; ev_trans releases them and dout),
     // then the saved activations' transposes.
+    const Bwd::Job dout_job = drop ? Bwd::Job{prec, tr.drop_out[par].p, H, doutT} : Bwd::Job{0, dcur, H, doutT};
+    const Bwd::Job dh1_job = drop ? Bwd::Job{prec, tr.drop_h1[par].p, H, dh1T} : Bwd::Job{0, dh1, H, dh1T};
     if (top)
-      RC(b.transposes({{prec, dwi, 2 * I, dwiT}, {0, dh1, H, dh1T}, {prec, dqkv, 3 * H, dqkvT}}, tr.side));
+      RC(b.transposes({{prec, dwi, 2 * I, dwiT}, dh1_job, {prec, dqkv, 3 * H, dqkvT}}, tr.side));
     else
-      RC(b.transposes({{0, dcur, H, doutT}, {prec, dwi, 2 * I, dwiT}, {0, dh1, H, dh1T}, {prec, dqkv, 3 * H, dqkvT}},
-                      tr.side));
-    HIPCHK(c, "colsum(norms)", launch_ln_bwd_colsum(lnp_mlp, T, H, grad(p + "mlp_norm.weight"), tr.side,
+      RC(b.transposes({dout_job, {prec, dwi, 2 * I, dwiT}, dh1_job, {prec, dqkv, 3 * H, dqkvT}}, tr.side));
+    if (!drop) HIPCHK(c, "colsum(norms)", launch_ln_bwd_colsum(lnp_mlp, T, H, grad(p + "mlp_norm.weight"), tr.side,
                                                     l > 0 ? lnp_attn : nullptr,
                                                     l > 0 ? grad(p + "attn_norm.weight") : nullptr));
     HIPCHK(c, "hipEventRecord", hipEventRecord(tr.ev_trans[par], tr.side));
@@ -514,6 +573,19 @@ int dn_set_trainable(dn_ctx *c, int train_from, int train_emb) {
   c->tr.train_from = std::min(train_from, c->cfg.layers);
   c->tr.train_emb = train_emb != 0;
   c->tr.have_forward = false;  // the kept activations depend on train_from
+  return DN_OK;
+}
+
+int dn_set_dropout(dn_ctx *c, float p, uint64_t seed, uint64_t step) {
+  if (!c) return DN_INVALID_ARG;
+  c->err.clear();
+  if (!c->tr.enabled) return fail(c, DN_INVALID_ARG, "decide_hip: dn_enable_training has not been called");
+  DropMask m{};
+  const blockchk::Refusal r = blockchk::mask("dn_set_dropout", p, seed, step, &m);
+  if (r.code) return fail(c, r.code, r.msg);
+  c->tr.drop.p = p;
+  c->tr.drop.seed = seed;
+  c->tr.drop.step = step;
   return DN_OK;
 }
 

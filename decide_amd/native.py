@@ -86,6 +86,7 @@ _SIGS = {
     "dn_evaluate": ([_vp, _i, _vp, _vp, _vp, _vp, _f64p, _c.c_int32, _i, _f64p, _vp, _f64p, _f64p], _i),
     "dn_enable_training": ([_vp], _i),
     "dn_set_trainable": ([_vp, _i, _i], _i),
+    "dn_set_dropout": ([_vp, _f, _u64, _u64], _i),
     "dn_forward_train": ([_vp, _i, _i32p, _i32p, _i32p, _i32p, _i32p, _i32p, _f32p, _i], _i),
     "dn_backward": ([_vp, _f32p, _i], _i),
     "dn_zero_grad": ([_vp], _i),

@@ -37,6 +37,11 @@ class TrainEngine(Engine):
         """gpunn.(*Model).SetTrainable (internal/gpunn/model.go:155-171)."""
         check(lib.dn_set_trainable(self._h, int(train_from), int(bool(train_emb))), self._h)
 
+    def set_dropout(self, p: float, seed: int = 0, step: int = 0) -> None:
+        """dn_set_dropout: dropout of every sub-layer's output in the training forwards that
+        follow; step: the number of forwards already made with this seed (a resumed run)."""
+        check(lib.dn_set_dropout(self._h, float(p), int(seed), int(step)), self._h)
+
     def infer(self, batch: Seq[Sequence]) -> np.ndarray:
         return Engine.forward(self, batch)
 

@@ -401,6 +401,21 @@ int dn_enable_training(dn_ctx *ctx);
  * (internal/train/optim.go:31-65). */
 int dn_set_trainable(dn_ctx *ctx, int train_from, int train_emb);
 
+/* Dropout of the sub-layers' outputs in the training forwards that follow
+ * (inference never drops): Wo's and MlpWo's products of every layer pass
+ * through dn_dropout_device's dropout (p in [0, 1], its mask rule and
+ * generator) on their way into the residual stream. The masks are never
+ * stored: element (token t of the batch, column c) after layer l's attention
+ * (site 0) or MLP (site 1) has row t, column c, this seed and the offset
+ * forward * 2 * layers + 2 * l + site, where `forward` is `step` in the next
+ * dn_forward_train and one more in each after it while p > 0. dn_backward
+ * regenerates the masks of its forward, whatever was set since. A resumed run
+ * passes the number of forwards already made. The default is p = 0 (no
+ * dropout, the kernels without it). Needs dn_enable_training;
+ * dn_set_config clears it. No counterpart in the reference, which trains
+ * without dropout. */
+int dn_set_dropout(dn_ctx *ctx, float p, uint64_t seed, uint64_t step);
+
 /* Forward that keeps the activations dn_backward needs (for layers >=
  * train_from). Arguments and validation as dn_forward. Replaces
  * gpunn.(*Model).Forward (internal/gpunn/model.go:204-330) and

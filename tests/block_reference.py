@@ -5,11 +5,12 @@ import numpy as np
 U = 2.0 ** -24  # half a step of fp32, relative
 # Half a step of each type relative to a value, and its smallest subnormal's half.
 HALF = {"fp32": (2.0 ** -24, 2.0 ** -150), "bf16": (2.0 ** -8, 2.0 ** -134), "fp16": (2.0 ** -11, 2.0 ** -25)}
-# Longest chain of fp32 additions in a row's sum: up to 128 elements in one
-# thread, then a tree over 64 lanes (6) and up to 16 waves.
+# Longest chain of fp32 additions in a row's sum: 128 are allowed for a thread's
+# elements (kernels hold 16 to 24), a tree over 64 lanes (6) and up to 16 waves.
 K = 160
-# And in a column's sum over the rows: rows of one thread and row groups of a
-# workgroup (at most 128 in these tests' sizes), then up to 512 partial sums.
+# And in a column's sum over the rows: 128 for the rows of one thread and the
+# waves of a workgroup in these tests' sizes, 512 for the partial sums (a
+# thread adds at most 12 of the 768, and 16 more join the threads).
 KR = 640
 
 
@@ -60,7 +61,7 @@ def norm_grad(dy, x, w, mean, rstd):
 
 
 def rounding(y, dtype):
-    """Half a step of dtype at y, doubled by nothing: what one rounding may move it."""
+    """Half a step of dtype at y: what one rounding may move it."""
     rel, least = HALF[dtype]
     return np.abs(y) * rel + least
 

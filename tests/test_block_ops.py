@@ -229,7 +229,7 @@ def test_workspace_sizes():
 
     for rows, cols in ((0, 1), (1, 1), (7, 768), (12288, 768), (2 ** 31 - 1, 16384)):
         n = Engine.norm_backward_workspace(rows, cols)
-        assert 0 <= n <= 512 * 2 * cols * 4 and n % 4 == 0
+        assert 0 <= n <= 768 * 2 * cols * 4 and n % 4 == 0
     for rows, cols in ((-1, 8), (8, 0), (8, 16385), (2 ** 31, 8)):
         with pytest.raises(ValueError):
             Engine.norm_backward_workspace(rows, cols)
