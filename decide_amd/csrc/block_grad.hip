@@ -8,18 +8,66 @@ namespace {
 // Workgroups of the gradient, each with partial sums of its own that cost a
 // slice of the workspace to write and to read again: up to three per CU while
 // they make 16 waves together, one for wide rows.
+// Calls of at most this many rows sum each column over all of them in
+// workgroups beside those of the rows: one launch instead of two.
+constexpr int64_t kSmallRows = 256;
+
 int row_parts(int64_t rows, int cols, int rows_per_group, int threads) {
   const int most = 256 * (cols > 4096 ? 1 : std::clamp(1024 / threads, 1, 3));
   return (int)std::min<int64_t>(most, (rows + rows_per_group - 1) / rows_per_group);
 }
 
-// All gradients in one pass over rows held in registers: with xh = (h - mean) rstd and g = dy w,
-// dres = dh + rstd (g - mean(g) - xh mean(g xh)) and dx = dropout's gradient of
-// it (the forward's mask and scale), from the unrounded sum. Each thread adds
-// dy xh and dy of its columns over its rows; a workgroup's sums go to its
-// slice of the workspace, [2][cols].
-template <class D, class S, class X, bool BOUNDARY, class Shape>
-__global__ __launch_bounds__(Shape::MAXT) void norm_grad_kernel(NormGradArgs a) {
+// Floats between the sums of a workgroup's dw and db, and of one workgroup and
+// the next: whole float4s, the last one's rest unused.
+__host__ __device__ constexpr int sum_stride(int cols) { return (cols + 3) / 4 * 4; }
+
+// dw and db of 32 columns over all rows (of few), by one workgroup: its threads
+// share the rows, eight loaded at a time, and their sums are added in order.
+template <class D, class S>
+__device__ __forceinline__ void column_sums(const NormGradArgs &a, int slab) {
+  constexpr int COLS = 32, BATCH = 8;
+  __shared__ float lds[2][1024 / COLS][COLS + 1];
+  const int i = threadIdx.x % COLS, k = threadIdx.x / COLS, step = blockDim.x / COLS, rows = (int)a.rows;
+  const int c = slab * COLS + i, at = min(c, a.cols - 1);
+  float sw = 0.0f, sb = 0.0f;
+  for (int r = k; r < rows; r += step * BATCH) {
+    float dy[BATCH], h[BATCH], mean[BATCH], rstd[BATCH];
+#pragma unroll
+    for (int j = 0; j < BATCH; j++) {
+      const int64_t row = min(r + j * step, rows - 1);
+      dy[j] = (float)((const D *)a.dy)[row * a.lddy + at];
+      h[j] = (float)((const S *)a.h)[row * a.ldh + at];
+      mean[j] = a.mean[row];
+      rstd[j] = a.rstd[row];
+    }
+#pragma unroll
+    for (int j = 0; j < BATCH; j++) {
+      if (r + j * step >= rows) break;
+      sw += dy[j] * ((h[j] - mean[j]) * rstd[j]);
+      sb += dy[j];
+    }
+  }
+  lds[0][k][i] = sw;
+  lds[1][k][i] = sb;
+  __syncthreads();
+  if (k >= 2 || c >= a.cols) return;
+  float *to = k ? a.db : a.dw;
+  if (!to) return;
+  float s = 0.0f;
+  for (int j = 0; j < step; j++) s += lds[k][j][i];
+  to[c] = a.accumulate ? to[c] + s : s;
+}
+
+// All gradients in one pass over rows held in registers: with xh = (h - mean)
+// rstd and g = dy w, dres = dh + rstd (g - mean(g) - xh mean(g xh)) and dx =
+// dropout's gradient of it (the forward's mask and scale), from the unrounded
+// sum. Each thread adds dy xh and dy of its columns over its rows; a
+// workgroup's sums go to its slice of the workspace. SMALL: the
+// workgroups past `groups` sum the columns instead.
+template <class D, class S, class X, bool BOUNDARY, bool SMALL, class Shape>
+__global__ __launch_bounds__(Shape::MAXT) void norm_grad_kernel(NormGradArgs a, int groups) {
+  if constexpr (SMALL)
+    if ((int)blockIdx.x >= groups) return column_sums<D, S>(a, blockIdx.x - groups);
   constexpr int VEC = Shape::VEC, LPR = Shape::LPR, VPT = Shape::VPT;
   constexpr bool WAVES = LPR == 0;
   // The widest rows' threads have 128 registers: dh is read after the row's sums there.
@@ -34,7 +82,7 @@ __global__ __launch_bounds__(Shape::MAXT) void norm_grad_kernel(NormGradArgs a) 
     for (int i = 0; i < VEC; i++) sw[j][i] = 0.0f, sb[j][i] = 0.0f;
   int turn = 0;
   for (int64_t row = row_of<LPR>((int64_t)blockIdx.x * Shape::ROWS); row < a.rows;
-       row += (int64_t)gridDim.x * Shape::ROWS, turn ^= 1) {
+       row += (int64_t)groups * Shape::ROWS, turn ^= 1) {
     // The weights are read again for every row (from the caches): held, they
     // would cost the registers of a wave per SIMD.
     const float *weight = a.w;
@@ -104,14 +152,15 @@ __global__ __launch_bounds__(Shape::MAXT) void norm_grad_kernel(NormGradArgs a) 
       }
     }
   }
-  if (!a.work) return;
-  float *out = a.work + (int64_t)blockIdx.x * 2 * cols;
+  if (SMALL || !a.work) return;
+  const int stride = sum_stride(cols);
+  float *out = a.work + (int64_t)blockIdx.x * 2 * stride;
   if constexpr (WAVES) {
 #pragma unroll
     for (int j = 0; j < VPT; j++) {
       const int c = VEC * (lane + j * lpr);
-      store<float, VEC>(out, c, cols, sw[j]);
-      store<float, VEC>(out + cols, c, cols, sb[j]);
+      if (a.dw) store<float, VEC>(out, c, cols, sw[j]);
+      if (a.db) store<float, VEC>(out + stride, c, cols, sb[j]);
     }
   } else {
     // Rows of one wave in registers, then the four waves through LDS in order.
@@ -139,42 +188,52 @@ __global__ __launch_bounds__(Shape::MAXT) void norm_grad_kernel(NormGradArgs a) 
       }
       __syncthreads();
     };
-    join(sw, out);
-    join(sb, out + cols);
+    if (a.dw) join(sw, out);
+    if (a.db) join(sb, out + stride);
   }
 }
 
-// The workgroups' sums in order: blockIdx.y 0 dw, 1 db; 16 columns of a
-// workgroup, 64 threads each, whose loads are made eight at a time.
+// The workgroups' sums in order: blockIdx.y 0 dw, 1 db; 32 columns of a
+// workgroup, four per thread, the parts shared by 128 threads that load eight
+// at a time; a wave's sums in registers, then the waves' through LDS.
 __global__ __launch_bounds__(1024) void norm_join_kernel(NormGradArgs a, int parts) {
-  constexpr int COLS = 16, SPLIT = 1024 / COLS, BATCH = 8;
-  __shared__ float lds[SPLIT][COLS + 1];
+  constexpr int COLS = 32, SPLIT = 128, BATCH = 8;
+  __shared__ float lds[16][COLS];
   float *to = blockIdx.y ? a.db : a.dw;
   if (!to) return;
-  const int i = threadIdx.x % COLS, c = blockIdx.x * COLS + i, k = threadIdx.x / COLS;
-  const float *from = a.work + (int64_t)blockIdx.y * a.cols + min(c, a.cols - 1);
-  float s = 0;
-  for (int p = k; p < parts; p += SPLIT * BATCH) {
-    float v[BATCH];
+  const int i = threadIdx.x % 8, k = threadIdx.x / 8, c = blockIdx.x * COLS + 4 * i;
+  const int stride = sum_stride(a.cols);
+  const float *from = a.work + (int64_t)blockIdx.y * stride;
+  float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (c < a.cols)
+    for (int p = k; p < parts; p += SPLIT * BATCH) {
+      float v[BATCH][4];
 #pragma unroll
-    for (int j = 0; j < BATCH; j++) v[j] = from[(int64_t)min(p + j * SPLIT, parts - 1) * 2 * a.cols];
+      for (int j = 0; j < BATCH; j++)
+        __builtin_memcpy(v[j], from + (int64_t)min(p + j * SPLIT, parts - 1) * 2 * stride + c, sizeof(v[j]));
 #pragma unroll
-    for (int j = 0; j < BATCH; j++) s += p + j * SPLIT < parts ? v[j] : 0.0f;
+      for (int j = 0; j < BATCH; j++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) s[e] += p + j * SPLIT < parts ? v[j][e] : 0.0f;
+    }
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    s[e] += __uint_as_float(dpp_u32<0x128>(__float_as_uint(s[e])));  // the other half of 16 lanes: row_ror 8
+    const auto q = __builtin_amdgcn_permlane16_swap(__float_as_uint(s[e]), __float_as_uint(s[e]), false, false);
+    s[e] = __uint_as_float(q[0]) + __uint_as_float(q[1]);
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(s[e]), __float_as_uint(s[e]), false, false);
+    s[e] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
   }
-  lds[k][i] = s;
-  __syncthreads();
-  if (k < 8) {
-    s = 0;
+  if ((threadIdx.x & 63) < 8)
 #pragma unroll
-    for (int j = 0; j < SPLIT / 8; j++) s += lds[k * (SPLIT / 8) + j][i];
-    lds[k * (SPLIT / 8)][i] = s;
-  }
+    for (int e = 0; e < 4; e++) lds[threadIdx.x >> 6][4 * i + e] = s[e];
   __syncthreads();
-  if (k == 0 && c < a.cols) {
-    s = 0;
+  const int out = blockIdx.x * COLS + threadIdx.x;
+  if (threadIdx.x < COLS && out < a.cols) {
+    float t = 0.0f;
 #pragma unroll
-    for (int j = 0; j < 8; j++) s += lds[j * (SPLIT / 8)][i];
-    to[c] = a.accumulate ? to[c] + s : s;
+    for (int j = 0; j < 16; j++) t += lds[j][threadIdx.x];
+    to[out] = a.accumulate ? to[out] + t : t;
   }
 }
 
@@ -197,16 +256,29 @@ hipError_t grad_launch(const NormGradArgs &args, hipStream_t s) {
   return with_grad_shape<vec_of<D, S, X>>(args.cols, [&](auto shape) {
     using Shape = decltype(shape);
     NormGradArgs a = args;
-    const int threads = Shape::threads(a.cols), parts = row_parts(a.rows, a.cols, Shape::ROWS, threads);
-    if (!a.dw && !a.db) a.work = nullptr;
-    if (parts > 0)
-      hipLaunchKernelGGL((norm_grad_kernel<D, S, X, BOUNDARY, Shape>), dim3(parts), dim3(threads), 0, s, a);
-    hipError_t e = hipGetLastError();
-    if (e == hipSuccess && (a.dw || a.db)) {
-      hipLaunchKernelGGL(norm_join_kernel, dim3((a.cols + 15) / 16, a.db ? 2 : 1), dim3(1024), 0, s, a, parts);
-      e = hipGetLastError();
+    const int threads = Shape::threads(a.cols);
+    const bool sums = a.dw || a.db;
+    if (a.rows <= kSmallRows) {
+      const int groups = ((int)a.rows + Shape::ROWS - 1) / Shape::ROWS, slabs = sums ? (a.cols + 31) / 32 : 0;
+      auto run = [&](int grid, int row_groups) {
+        if (grid > 0)
+          hipLaunchKernelGGL((norm_grad_kernel<D, S, X, BOUNDARY, true, Shape>), dim3(grid), dim3(threads), 0, s, a,
+                             row_groups);
+        return hipGetLastError();
+      };
+      // Where an output takes the place of what the sums read, the sums go first.
+      const bool over = a.dres == a.dy || a.dres == a.h || (BOUNDARY && (a.dx == a.dy || a.dx == a.h));
+      if (!over) return run(groups + slabs, groups);
+      const hipError_t e = run(slabs, 0);
+      return e == hipSuccess ? run(groups, groups) : e;
     }
-    return e;
+    const int parts = row_parts(a.rows, a.cols, Shape::ROWS, threads);
+    if (!sums) a.work = nullptr;
+    hipLaunchKernelGGL((norm_grad_kernel<D, S, X, BOUNDARY, false, Shape>), dim3(parts), dim3(threads), 0, s, a, parts);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || !sums) return e;
+    hipLaunchKernelGGL(norm_join_kernel, dim3((a.cols + 31) / 32, a.db ? 2 : 1), dim3(1024), 0, s, a, parts);
+    return hipGetLastError();
   });
 }
 
@@ -229,6 +301,7 @@ hipError_t boundary_grad_pick(int dy_type, int stream_type, int dx_type, const N
 
 // The larger of what calls with and without an fp32 array use.
 int64_t norm_grad_work(int64_t rows, int cols) {
+  if (rows <= kSmallRows) return 0;
   int parts = 0;
   auto most = [&](auto shape) {
     using Shape = decltype(shape);
@@ -237,7 +310,7 @@ int64_t norm_grad_work(int64_t rows, int cols) {
   };
   (void)with_grad_shape<4>(cols, most);
   (void)with_grad_shape<8>(cols, most);
-  return (int64_t)parts * 2 * cols;
+  return (int64_t)parts * 2 * sum_stride(cols);
 }
 
 hipError_t launch_norm_grad(int dy_type, int x_type, const NormGradArgs &a, hipStream_t s) {

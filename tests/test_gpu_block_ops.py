@@ -19,7 +19,7 @@ BOUNDARY_TYPES = [("fp32", "fp32", "fp32"), ("bf16", "fp32", "bf16"), ("fp16", "
 # workgroup's rows, the widest row.
 COLS = [1, 2, 3, 4, 5, 7, 8, 9, 31, 33, 100, 64, 127, 255, 256, 257, 384, 511, 512, 513, 768, 1000, 1023, 1024, 1025, 1152, 1536, 2047,
         2048, 2049, 4096, 4099, 6000, 8192, 8193, 6145, 9999, 12000, 16383, 16384]
-ROWS = [1, 2, 3, 5, 7, 8, 9, 16, 17, 31, 33, 64, 65, 203]
+ROWS = [1, 2, 3, 5, 7, 8, 9, 16, 17, 31, 33, 64, 65, 203, 300]
 GUARD = 7.25  # what stands around an array's columns; exact in every type
 
 
