@@ -5,11 +5,16 @@
 
 namespace {
 
-// Workgroups of the gradient, each with partial sums of its own that cost a
-// slice of the workspace to write and to read again: up to three per CU while
-// they make 16 waves together, one for wide rows.
+// Workgroups of the gradient of many rows, each with partial sums of its own
+// that cost a slice of the workspace to write and to read again: up to three
+// per CU while they make 16 waves together (12,288 x 768: 768 workgroups 37.4
+// us, 512 39.0, 1,024 38.2), one past 4,096 columns (4,096 x 8,192: 256
+// workgroups 75 us, 512 82).
 // Calls of at most this many rows sum each column over all of them in
-// workgroups beside those of the rows: one launch instead of two.
+// workgroups beside those of the rows: one launch (of ~3.5 us on the host)
+// instead of two, for a second read of dy and h from the caches. One launch and
+// two: 256 x 768 8.4 and 10.3 us, 512 x 768 11.7 and 10.2, 1,024 x 768 40 and 11;
+// 256 x 8,192 8.6 and 19.3.
 constexpr int64_t kSmallRows = 256;
 
 int row_parts(int64_t rows, int cols, int rows_per_group, int threads) {
@@ -64,6 +69,11 @@ __device__ __forceinline__ void column_sums(const NormGradArgs &a, int slab) {
 // sum. Each thread adds dy xh and dy of its columns over its rows; a
 // workgroup's sums go to its slice of the workspace. SMALL: the
 // workgroups past `groups` sum the columns instead.
+//
+// HBM-bound: 12,288 x 768 (dy bf16, stream fp32) 18.7 us, with dropout's gradient
+// 30.2, both 5 TB/s; the sums that follow (norm_join_kernel) 4 to 5 us more. The
+// rows of a workgroup come from a loop, since its sums live in registers; three
+// to four waves per SIMD cover the loop's wait for its stores.
 template <class D, class S, class X, bool BOUNDARY, bool SMALL, class Shape>
 __global__ __launch_bounds__(Shape::MAXT) void norm_grad_kernel(NormGradArgs a, int groups) {
   if constexpr (SMALL)
@@ -238,7 +248,8 @@ __global__ __launch_bounds__(1024) void norm_join_kernel(NormGradArgs a, int par
 }
 
 // The gradient's threads also hold two sums per column, so its shapes have
-// fewer columns a thread than the forward's.
+// fewer columns a thread than the forward's. Past 4,096 columns two vectors of
+// eight in 512 threads (4,096 x 8,192: 69 us) before one in 1,024 (76).
 template <int WIDE, class F>
 hipError_t with_grad_shape(int cols, F f) {
   if (cols < WIDE) return f(RowShape<1, 8, 1>{});

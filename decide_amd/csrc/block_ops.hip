@@ -10,8 +10,17 @@ constexpr int kThreads = 256;
 // Most workgroups of a launch (fewer than 2^32 threads); more rows take several.
 constexpr int kGrid = 1 << 20;
 
-// LayerNorm of rows held in registers. BOUNDARY: the row is res + dropout(x),
-// stored to h.
+// LayerNorm of rows held in registers: one read of each input, one write of
+// each output. BOUNDARY: the row is res + dropout(x), stored to h.
+//
+// HBM-bound from a few thousand rows on; a launch's latency below. A row per
+// wave (or part of one) up to 1,024 columns, a row per workgroup above, one row
+// per thread group and no loop over rows: loads and stores share one counter
+// (vmcnt), so that a loop's next row waits for this row's stores (32,768 x 768
+// with a row prefetched in a loop 58 us, without a loop 29.5, 5.1 TB/s, the
+// rate of a large copy; 12,288 rows with dropout 45 and 23.5, 4.8 TB/s). The
+// weights are read after the sums, not held: at most 64 registers, eight waves
+// per SIMD. 768 x 64 rows: 3.1 us on the GPU, 4.6 a call.
 template <class X, class S, class Y, bool BOUNDARY, class Shape>
 __global__ __launch_bounds__(Shape::MAXT) void norm_kernel(NormArgs a, int64_t first) {
   constexpr int VEC = Shape::VEC, LPR = Shape::LPR, VPT = Shape::VPT;
@@ -93,12 +102,17 @@ __global__ __launch_bounds__(Shape::MAXT) void norm_kernel(NormArgs a, int64_t f
   }
 }
 
-// Elementwise, two vectors of VEC columns per thread: the launch's vectors i and
-// i + 64 of 128 that a wave takes, so that a wave's accesses are side by side. A
-// row has `per_row` generator blocks of eight columns, the last of `tail`; the
-// launch starts at block k0 of row r0. With VEC 4 (fp32 arrays) the two lanes
-// of a block share the generator's work as Columns::drop says. NARROW: rows of
-// less than eight columns, element by element.
+// Elementwise dropout. HBM-bound (32,768 x 1,152 bf16 29.4 us, 5.1 TB/s) with the
+// VALU 75% busy, most of it the generator's twenty 32 x 32 -> 64-bit products
+// per eight columns. No loop, for norm_kernel's reason (2,048 workgroups in a loop
+// 37.8 us); rows and blocks from one 32-bit division per vector.
+//
+// A thread takes a vector of eight columns, or (VEC 4, with an fp32 array) two of
+// four: the launch's vectors i and i + 64 of the 128 of a wave, so that a wave's
+// 16-byte accesses lie side by side (fp32 12 M elements 22.0 -> 20.2 us). The two
+// lanes of a generator block then share its work (drop_pair). A row has `per_row`
+// blocks of eight columns, the last of `tail`; the launch starts at block k0 of
+// row r0. NARROW: rows of less than eight columns, element by element.
 template <class X, class Y, bool RES, bool NARROW>
 __global__ __launch_bounds__(kThreads) void dropout_kernel(DropArgs a, uint32_t r0, uint32_t k0, uint32_t per_row,
                                                            uint32_t tail) {
@@ -184,6 +198,8 @@ hipError_t norm_launch(const NormArgs &a, hipStream_t s) {
     }
     return hipSuccess;
   };
+  // Vectors per thread past 1,024 columns: 1, 2 and 3 of eight, 2, 3 and 4 of
+  // four measured within 5% of each other; the most is what 16,384 columns need.
   if constexpr (vec_of<X, S, Y> == 8) {
     if (a.cols < 8) return run(RowShape<1, 8, 1>{});
     return pick_shape<RowShape<8, 8, 1>, RowShape<8, 16, 1>, RowShape<8, 32, 1>, RowShape<8, 32, 2>, RowShape<8, 32, 3>,

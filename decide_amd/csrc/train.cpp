@@ -25,6 +25,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstring>
+#include <exception>
 #include <initializer_list>
 #include <numeric>
 #include <string>
@@ -581,8 +582,12 @@ int dn_set_dropout(dn_ctx *c, float p, uint64_t seed, uint64_t step) {
   c->err.clear();
   if (!c->tr.enabled) return fail(c, DN_INVALID_ARG, "decide_hip: dn_enable_training has not been called");
   DropMask m{};
-  const blockchk::Refusal r = blockchk::mask("dn_set_dropout", p, seed, step, &m);
-  if (r.code) return fail(c, r.code, r.msg);
+  try {
+    const blockchk::Refusal r = blockchk::mask("dn_set_dropout", p, seed, step, &m);
+    if (r.code) return fail(c, r.code, r.msg);
+  } catch (const std::exception &) {
+    return DN_OUT_OF_MEMORY;
+  }
   c->tr.drop.p = p;
   c->tr.drop.seed = seed;
   c->tr.drop.step = step;

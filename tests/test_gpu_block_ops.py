@@ -329,6 +329,26 @@ def test_boundary_many_rows(eng):
         check_norm(eng, rng, rows, cols, "fp32", "bf16")
 
 
+def test_more_rows_than_a_launch_takes(eng):
+    """A row per workgroup and 2^20 workgroups a launch: rows on both sides of the second launch's first."""
+    rows, cols = 2 ** 20 + 5, 1040
+    x = torch.zeros(rows, cols, dtype=torch.bfloat16, device="cuda")
+    res, h, y = (torch.zeros_like(x) for _ in range(3))
+    at = [0, 1, 2 ** 20 - 1, 2 ** 20, rows - 1]
+    rng = np.random.default_rng(77)
+    x[at] = torch.from_numpy(rng.standard_normal((5, cols))).to(torch.bfloat16).cuda()
+    mean, rstd = torch.zeros(rows, device="cuda"), torch.zeros(rows, device="cuda")
+    eng.dropout_add_norm_device("bf16", "bf16", "bf16", rows, cols, ptr(x), cols, ptr(res), cols, 0.25, 9, 8, None, None,
+                                EPS, ptr(h), cols, ptr(y), cols, ptr(mean), ptr(rstd))
+    keep = ref.keep_scale(np.array(at), cols, 0.25, 9, 8)
+    want = ref.drop(f64(x[at]), keep)
+    within(h[at], want, 2 * ref.U * np.abs(want) + ref.rounding(np.abs(want) * (1 + 2 * ref.U), "bf16"), "h")
+    n = ref.norm(f64(h[at]), None, None, EPS)
+    bounds = ref.norm_bounds(f64(h[at]), None, None, EPS, *n, "bf16")
+    for got, wanted, bound in zip((y[at], mean[at], rstd[at]), n, bounds):
+        within(got, wanted, bound, "rows")
+
+
 def test_no_rows(eng):
     """No rows: nothing is touched, and the sums are the empty sum (stored, or added to what is there)."""
     g = torch.full((16,), GUARD, device="cuda")
