@@ -207,8 +207,7 @@ hipError_t norm_launch(const NormArgs &a, hipStream_t s) {
   } else {
     if (a.cols < 4) return run(RowShape<1, 8, 1>{});
     return pick_shape<RowShape<4, 8, 1>, RowShape<4, 16, 1>, RowShape<4, 32, 1>, RowShape<4, 64, 1>, RowShape<4, 64, 2>,
-                      RowShape<4, 64, 3>, RowShape<4, 64, 4>, RowShape<4, 0, 4, 1024>>(a.cols,
-                                                                                                              run);
+                      RowShape<4, 64, 3>, RowShape<4, 64, 4>, RowShape<4, 0, 4, 1024>>(a.cols, run);
   }
 }
 

@@ -39,12 +39,12 @@ __device__ __forceinline__ uint4 philox(uint32_t c0, uint32_t c1, uint32_t c2, u
 }
 
 // Drops elements in place (the scale of the others is the caller's, one
-// multiply-add with what they are added to), from the generator's words that hold their 16-bit
-// draws: element j takes half j % 2 (0 low) of word j / 2. A dropped element
-// is 0 whatever it was (also an infinity or a NaN), so it is selected, not
-// multiplied. A half is at least the threshold t > 0 where its word, with that
-// half in the upper bits, is above 65536 t - 1: the lower bits only add, and
-// at t = 65536 nothing is above 2^32 - 1.
+// multiply-add with what they are added to), from the generator's words that
+// hold their 16-bit draws: element j takes half j % 2 (0 low) of word j / 2. A
+// dropped element is 0 whatever it was (also an infinity or a NaN), so it is
+// selected, not multiplied. A half is at least the threshold t > 0 where its
+// word, with that half in the upper bits, is above 65536 t - 1: the lower bits
+// only add, and at t = 65536 nothing is above 2^32 - 1.
 __device__ __forceinline__ float keep(const DropMask &m, uint32_t upper, float v) {
   return upper > (m.threshold << 16) - 1u ? v : 0.0f;
 }

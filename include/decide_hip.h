@@ -463,21 +463,24 @@ int dn_set_adam_step(dn_ctx *ctx, int step);
 
 /* ---- Training-block operators on device arrays ---------------------------
  * LayerNorm, dropout and the residual boundary made of both, each with its
- * gradient: what dn_forward_train runs inside the model, as operators of their
- * own. They need an open context only (no configuration), run asynchronously
- * on its stream, allocate and wait for nothing, and may be captured into a
- * graph; replays of graphs that share a d_work must not overlap. The current
- * device of the calling thread is left as it was.
+ * gradient, at any width and in any of the library's types; training with
+ * dropout (dn_set_dropout) runs on them. They need an open context only (no
+ * configuration), run asynchronously on its stream, allocate and wait for
+ * nothing, and may be captured into a graph; calls (and replays) that share a
+ * d_work must not overlap. The current device of the calling thread is left as
+ * it was.
  * Arrays are [rows x cols], row r at base + r * ld elements (ld >= cols; any
  * value for a single row), aligned to their elements: odd widths, strides and
  * offsets are ordinary. *_type are DN_PRECISION_* codes; the arithmetic and
- * every sum are fp32, and each output is rounded once. A call's 16-bit arrays are all of one type. Weights, biases,
- * their gradients and row statistics are fp32. An output may be an input's
- * very array (the same address, stride and element size); any other overlap
- * with an output is refused (DN_INVALID_ARG), as are NULL, misaligned or
- * too-narrow arrays. rows may be 0. Norms take 1 to 16,384 columns
- * (DN_UNSUPPORTED beyond). No counterpart in the reference, whose model has no
- * dropout and whose LayerNorm (internal/nn/ops.go:63-138) runs inside it. */
+ * every sum are fp32, and each output is rounded once. A call's 16-bit arrays
+ * are all of one type. Weights, biases, their gradients and row statistics are
+ * fp32. An output may be an input's very array (the same address, stride and
+ * element size); any other overlap with an output is refused (DN_INVALID_ARG),
+ * as are NULL, misaligned or too-narrow arrays. rows may be 0. Norms take 1 to
+ * 16,384 columns (DN_UNSUPPORTED beyond). A row with an infinity or a NaN
+ * gives NaN in that row and, through dw and db, in their sums. No counterpart
+ * in the reference, whose model has no dropout and whose LayerNorm
+ * (internal/nn/ops.go:63-138) runs inside it. */
 
 /* y = (x - mean) * rstd * w + b over each row, mean = sum x / cols, rstd =
  * 1 / sqrt(sum (x - mean)^2 / cols + eps), eps > 0. d_w NULL: 1, d_b NULL: 0.
@@ -488,7 +491,8 @@ int dn_layer_norm_device(dn_ctx *ctx, int x_type, int y_type, int64_t rows, int 
                          float *d_rstd);
 
 /* Bytes of d_work for the two backward calls that follow, when they compute a
- * weight or bias gradient; -1 for sizes they do not take. */
+ * weight or bias gradient (0: none is needed, d_work may be NULL); -1 for sizes
+ * they do not take. */
 int64_t dn_norm_backward_workspace(int64_t rows, int cols);
 
 /* The gradients of dn_layer_norm_device from dy, x and the kept mean and rstd:

@@ -617,6 +617,56 @@ def test_other_stream_and_graph(eng):
         eng.set_stream(before)
 
 
+def test_two_contexts_at_once():
+    """Two contexts without a model, each on a stream of its own, give what each gives alone."""
+    import ctypes
+
+    from decide_amd import native
+
+    lib, rows, cols = native.lib, 4097, 768
+    handles, streams = [], [torch.cuda.Stream() for _ in range(2)]
+    try:
+        for s in streams:
+            h = ctypes.c_void_p()
+            if lib.dn_open(0, ctypes.byref(h)) == native.DN_NO_GPU:
+                pytest.skip("no GPU")
+            handles.append(h)
+            assert lib.dn_set_stream(h, s.cuda_stream) == 0
+        n = lib.dn_norm_backward_workspace(rows, cols)
+        data = []
+        for k in range(2):
+            g = torch.Generator(device="cuda").manual_seed(k)
+            d = {name: torch.randn(rows, cols, generator=g, device="cuda") for name in ("dy", "dh", "h", "dres", "dx")}
+            d["mean"], d["rstd"] = d["h"].mean(1), 1 / d["h"].std(1)
+            d["dw"], d["work"] = torch.zeros(cols, device="cuda"), torch.zeros(n, dtype=torch.uint8, device="cuda")
+            data.append(d)
+
+        def call(h, d, k):
+            q = {name: t.data_ptr() for name, t in d.items()}
+            assert lib.dn_dropout_add_norm_backward_device(
+                h, 0, 0, 0, rows, cols, q["dy"], cols, q["dh"], cols, q["h"], cols, 0.1, 5 + k, 6, None, q["mean"],
+                q["rstd"], q["dres"], cols, q["dx"], cols, q["dw"], None, 0, q["work"], n) == 0
+
+        alone = []
+        for k in range(2):
+            torch.cuda.synchronize()
+            call(handles[k], data[k], k)
+            torch.cuda.synchronize()
+            alone.append([data[k][o].clone() for o in ("dres", "dx", "dw")])
+            for o in ("dres", "dx", "dw"):
+                data[k][o].zero_()
+        torch.cuda.synchronize()
+        for _ in range(10):
+            for k in range(2):
+                call(handles[k], data[k], k)
+        torch.cuda.synchronize()
+        for k in range(2):
+            assert all(torch.equal(data[k][o], a) for o, a in zip(("dres", "dx", "dw"), alone[k]))
+    finally:
+        for h in handles:
+            lib.dn_close(h)
+
+
 def test_refusals_reach_the_caller(eng):
     """A refused call names its reason and writes nothing."""
     from decide_amd import InvalidArgument, Unsupported
