@@ -219,7 +219,7 @@ def test_boundary_gradient_sizes(eng, cols):
                    accumulate=k % 2 == 1)
 
 
-@pytest.mark.parametrize("rows", [1000, 4097, 12288])
+@pytest.mark.parametrize("rows", [64, 256, 257, 1000, 4097, 12288])
 def test_gradient_many_rows(eng, rows):
     """Rows past every workgroup's first ones; the sums over them, and each alone."""
     rng = np.random.default_rng(rows)
@@ -363,11 +363,12 @@ def test_no_rows(eng):
     assert bool((g == GUARD).all())
 
 
-@pytest.mark.parametrize("cols", [100, 768, 2049])
-def test_in_place(eng, cols):
+@pytest.mark.parametrize("rows", [37, 300])
+@pytest.mark.parametrize("cols", [5, 100, 768, 2049, 12001])
+def test_in_place(eng, cols, rows):
     """An output in an input's array gives the bits of the call with arrays of its own."""
     rng = np.random.default_rng(cols)
-    rows, p, seed, offset = 37, 0.2, 5, 6
+    p, seed, offset = 0.2, 5, 6
     v, r = stream_values(rng, rows, cols), stream_values(rng, rows, cols)
     w = vec(1 + 0.2 * rng.standard_normal(cols))
     x, res = Matrix(rows, cols, "bf16", v), Matrix(rows, cols, "bf16", r)
@@ -397,8 +398,12 @@ def test_in_place(eng, cols):
                                              cols, p, seed, offset, ptr(w), ptr(c["mean"]), ptr(c["rstd"]), dres.at,
                                              cols, dx.at, cols, ptr(dw), None, False, ptr(c["work"]), c["work_bytes"])
 
-    dw1, dw2 = torch.empty(cols, device="cuda"), torch.empty(cols, device="cuda")
+    dw1, dw2, dw3 = (torch.empty(cols, device="cuda") for _ in range(3))
     grad(c["dres"], c["dx"], c["dy"], c["dh"], dw1)
+    dy3 = Matrix(rows, cols, "bf16", c["dy"].view)
+    dx3 = Matrix(rows, cols, "bf16")
+    grad(dy3, dx3, dy3, c["dh"], dw3)
+    assert torch.equal(dy3.view, c["dres"].view) and torch.equal(dx3.view, c["dx"].view) and torch.equal(dw1, dw3)
     dy2, dh2 = Matrix(rows, cols, "bf16", c["dy"].view), Matrix(rows, cols, "bf16", c["dh"].view)
     grad(dh2, dy2, dy2, dh2, dw2)
     assert torch.equal(dh2.view, c["dres"].view) and torch.equal(dy2.view, c["dx"].view) and torch.equal(dw1, dw2)
@@ -445,6 +450,28 @@ def test_offsets_past_32_bits(eng):
         keep, scale = ref.keep_scale(np.zeros(1, np.int64), c, 0.5, 3, 4)
         assert np.array_equal(buf[c0: c0 + len(c)].float().cpu().numpy(), (keep[0] * scale).astype(np.float32)), c0
     assert float(buf[long]) == 0.0 or ld < long + 1
+
+
+def test_gradient_of_rows_that_are_not_finite(eng):
+    """A NaN or an infinity in dy, dh or h makes its own row's gradient NaN (or infinite) and the sums of its
+    column, and nothing else; dropped elements of dx are 0 all the same."""
+    for rows, cols in ((40, 96), (400, 96), (40, 3001)):
+        rng = np.random.default_rng(rows + cols)
+        c = grad_case(rng, rows, cols, "fp32", "fp32", "fp32")
+        c["dy"].view[3, 5], c["dh"].view[7, 6], c["dy"].view[9, cols - 1] = float("nan"), float("inf"), float("-inf")
+        eng.dropout_add_norm_backward_device(
+            "fp32", "fp32", "fp32", rows, cols, c["dy"].at, cols, c["dh"].at, cols, c["h"].at, cols, 0.5, 1, 2, None,
+            ptr(c["mean"]), ptr(c["rstd"]), c["dres"].at, cols, c["dx"].at, cols, ptr(c["dw"]), ptr(c["db"]), False,
+            ptr(c["work"]), c["work_bytes"])
+        keep, _ = ref.keep_scale(rows, cols, 0.5, 1, 2)
+        dres, dx = c["dres"].f64(), c["dx"].f64()
+        bad = ~np.isfinite(dres)
+        assert bad[3].all() and bad[9].all() and bad[7].sum() == 1 and bad[7, 6] and dres[7, 6] == np.inf
+        bad[[3, 7, 9]] = False
+        assert not bad.any()
+        assert (dx[~keep] == 0).all() and np.array_equal(~np.isfinite(dx), keep & ~np.isfinite(dres))
+        for t in (c["dw"], c["db"]):
+            assert np.flatnonzero(~np.isfinite(f64(t)[:cols])).tolist() == [5, cols - 1]
 
 
 def test_equal_calls_give_equal_bits(eng):
@@ -553,11 +580,12 @@ def test_block_of_sublayers(eng):
         assert float((got.double().cpu() - want).norm() / want.norm()) < 1e-5
 
 
-def test_other_stream_and_graph(eng):
+@pytest.mark.parametrize("rows", [60, 515])
+def test_other_stream_and_graph(eng, rows):
     """The calls on another stream, captured into a graph and replayed on new inputs, with eager calls and
     synchronizations between the replays; two graphs with workspaces of their own replay side by side."""
     rng = np.random.default_rng(13)
-    rows, cols, p, seed, offset = 515, 768, 0.1, 31, 32
+    cols, p, seed, offset = 768, 0.1, 31, 32
     w = vec(1 + 0.2 * rng.standard_normal(cols))
     n = eng.norm_backward_workspace(rows, cols)
 
@@ -567,7 +595,7 @@ def test_other_stream_and_graph(eng):
                 "y": torch.zeros(rows, cols, **half), "mean": torch.zeros(rows, **f), "rstd": torch.zeros(rows, **f),
                 "dres": torch.zeros(rows, cols, **f), "dx": torch.zeros(rows, cols, **half),
                 "dw": torch.zeros(cols, **f), "db": torch.zeros(cols, **f),
-                "work": torch.zeros(n, dtype=torch.uint8, device="cuda")}
+                "work": torch.zeros(n + 16, dtype=torch.uint8, device="cuda")}
 
     def calls(a):
         q = {k: ptr(v) for k, v in a.items()}
