@@ -13,9 +13,13 @@ namespace {
 // Calls of at most this many rows sum each column over all of them in
 // workgroups beside those of the rows: one launch (of ~3.5 us on the host)
 // instead of two, for a second read of dy and h from the caches. One launch and
-// two: 256 x 768 8.4 and 10.3 us, 512 x 768 11.7 and 10.2, 1,024 x 768 40 and 11;
-// 256 x 8,192 8.6 and 19.3.
-constexpr int64_t kSmallRows = 256;
+// two: 256 x 768 8.3 and 10.8 us, 512 x 768 8.3 and 10.9, 768 x 768 11.0 and 10.8,
+// 1,024 x 768 13.7 and 10.9; 512 x 8,192 14.7 and 16.4, 1,024 x 8,192 27.7 and 26.9.
+constexpr int64_t kSmallRows = 512;
+// Columns of such a workgroup: few, so that many threads share the rows (512 x
+// 768: 8 columns 8.3 us, 16 8.6, 32 11.7), or 32 where the columns alone make
+// enough workgroups and narrow reads cost more (512 x 8,192: 30, 20 and 14.7).
+__host__ __device__ constexpr int slab_cols(int cols) { return cols <= 4096 ? 8 : 32; }
 
 int row_parts(int64_t rows, int cols, int rows_per_group, int threads) {
   const int most = 256 * (cols > 4096 ? 1 : std::clamp(1024 / threads, 1, 3));
@@ -26,11 +30,12 @@ int row_parts(int64_t rows, int cols, int rows_per_group, int threads) {
 // the next: whole float4s, the last one's rest unused.
 __host__ __device__ constexpr int sum_stride(int cols) { return (cols + 3) / 4 * 4; }
 
-// dw and db of 32 columns over all rows (of few), by one workgroup: its threads
-// share the rows, eight loaded at a time, and their sums are added in order.
-template <class D, class S>
+// dw and db of COLS columns over all rows (of few), by one workgroup: its
+// threads share the rows, eight loaded at a time, and their sums are added in
+// order.
+template <class D, class S, int COLS>
 __device__ __forceinline__ void column_sums(const NormGradArgs &a, int slab) {
-  constexpr int COLS = 32, BATCH = 8;
+  constexpr int BATCH = 8;
   __shared__ float lds[2][1024 / COLS][COLS + 1];
   const int i = threadIdx.x % COLS, k = threadIdx.x / COLS, step = blockDim.x / COLS, rows = (int)a.rows;
   const int c = slab * COLS + i, at = min(c, a.cols - 1);
@@ -59,6 +64,7 @@ __device__ __forceinline__ void column_sums(const NormGradArgs &a, int slab) {
   float *to = k ? a.db : a.dw;
   if (!to) return;
   float s = 0.0f;
+#pragma unroll 8
   for (int j = 0; j < step; j++) s += lds[k][j][i];
   to[c] = a.accumulate ? to[c] + s : s;
 }
@@ -77,7 +83,10 @@ __device__ __forceinline__ void column_sums(const NormGradArgs &a, int slab) {
 template <class D, class S, class X, bool BOUNDARY, bool SMALL, class Shape>
 __global__ __launch_bounds__(Shape::MAXT) void norm_grad_kernel(NormGradArgs a, int groups) {
   if constexpr (SMALL)
-    if ((int)blockIdx.x >= groups) return column_sums<D, S>(a, blockIdx.x - groups);
+    if ((int)blockIdx.x >= groups) {
+      const int slab = blockIdx.x - groups;
+      return slab_cols(a.cols) == 8 ? column_sums<D, S, 8>(a, slab) : column_sums<D, S, 32>(a, slab);
+    }
   constexpr int VEC = Shape::VEC, LPR = Shape::LPR, VPT = Shape::VPT;
   constexpr bool WAVES = LPR == 0;
   // The widest rows' threads have 128 registers: dh is read after the row's sums there.
@@ -270,7 +279,8 @@ hipError_t grad_launch(const NormGradArgs &args, hipStream_t s) {
     const int threads = Shape::threads(a.cols);
     const bool sums = a.dw || a.db;
     if (a.rows <= kSmallRows) {
-      const int groups = ((int)a.rows + Shape::ROWS - 1) / Shape::ROWS, slabs = sums ? (a.cols + 31) / 32 : 0;
+      const int groups = ((int)a.rows + Shape::ROWS - 1) / Shape::ROWS, slab = slab_cols(a.cols);
+      const int slabs = sums ? (a.cols + slab - 1) / slab : 0;
       auto run = [&](int grid, int row_groups) {
         if (grid > 0)
           hipLaunchKernelGGL((norm_grad_kernel<D, S, X, BOUNDARY, true, Shape>), dim3(grid), dim3(threads), 0, s, a,

@@ -19,7 +19,7 @@ BOUNDARY_TYPES = [("fp32", "fp32", "fp32"), ("bf16", "fp32", "bf16"), ("fp16", "
 # workgroup's rows, the widest row.
 COLS = [1, 2, 3, 4, 5, 7, 8, 9, 31, 33, 100, 64, 127, 255, 256, 257, 384, 511, 512, 513, 768, 1000, 1023, 1024, 1025, 1152, 1536, 2047,
         2048, 2049, 4096, 4099, 6000, 8192, 8193, 6145, 9999, 12000, 16383, 16384]
-ROWS = [1, 2, 3, 5, 7, 8, 9, 16, 17, 31, 33, 64, 65, 203, 300]
+ROWS = [1, 2, 3, 5, 7, 8, 9, 16, 17, 31, 33, 64, 65, 203, 530]
 GUARD = 7.25  # what stands around an array's columns; exact in every type
 
 
@@ -219,7 +219,7 @@ def test_boundary_gradient_sizes(eng, cols):
                    accumulate=k % 2 == 1)
 
 
-@pytest.mark.parametrize("rows", [64, 256, 257, 1000, 4097, 12288])
+@pytest.mark.parametrize("rows", [64, 257, 512, 513, 1000, 4097, 12288])
 def test_gradient_many_rows(eng, rows):
     """Rows past every workgroup's first ones; the sums over them, and each alone."""
     rng = np.random.default_rng(rows)
@@ -363,7 +363,7 @@ def test_no_rows(eng):
     assert bool((g == GUARD).all())
 
 
-@pytest.mark.parametrize("rows", [37, 300])
+@pytest.mark.parametrize("rows", [37, 530])
 @pytest.mark.parametrize("cols", [5, 100, 768, 2049, 12001])
 def test_in_place(eng, cols, rows):
     """An output in an input's array gives the bits of the call with arrays of its own."""
@@ -455,7 +455,7 @@ def test_offsets_past_32_bits(eng):
 def test_gradient_of_rows_that_are_not_finite(eng):
     """A NaN or an infinity in dy, dh or h makes its own row's gradient NaN (or infinite) and the sums of its
     column, and nothing else; dropped elements of dx are 0 all the same."""
-    for rows, cols in ((40, 96), (400, 96), (40, 3001)):
+    for rows, cols in ((40, 96), (700, 96), (40, 3001), (40, 5001)):
         rng = np.random.default_rng(rows + cols)
         c = grad_case(rng, rows, cols, "fp32", "fp32", "fp32")
         c["dy"].view[3, 5], c["dh"].view[7, 6], c["dy"].view[9, cols - 1] = float("nan"), float("inf"), float("-inf")
