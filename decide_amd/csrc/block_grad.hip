@@ -259,6 +259,9 @@ __global__ __launch_bounds__(1024) void norm_join_kernel(NormGradArgs a, int par
 // The gradient's threads also hold two sums per column, so its shapes have
 // fewer columns a thread than the forward's. Past 4,096 columns two vectors of
 // eight in 512 threads (4,096 x 8,192: 69 us) before one in 1,024 (76).
+// With an fp32 array three vectors of four reach 12,288 columns without a
+// spilled register, where four spill up to 39 (boundary, bf16 with an fp32
+// stream, 8,200 columns: 52 and 88 us); four are what 16,384 columns need.
 template <int WIDE, class F>
 hipError_t with_grad_shape(int cols, F f) {
   if (cols < WIDE) return f(RowShape<1, 8, 1>{});
@@ -268,7 +271,7 @@ hipError_t with_grad_shape(int cols, F f) {
   else
     return pick_shape<RowShape<4, 8, 1>, RowShape<4, 16, 1>, RowShape<4, 32, 1>, RowShape<4, 64, 1>, RowShape<4, 64, 2>,
                       RowShape<4, 64, 3>, RowShape<4, 64, 4>, RowShape<4, 0, 1, 512>, RowShape<4, 0, 2, 1024>,
-                      RowShape<4, 0, 4, 1024>>(cols, f);
+                      RowShape<4, 0, 3, 1024>, RowShape<4, 0, 4, 1024>>(cols, f);
 }
 
 template <class D, class S, class X, bool BOUNDARY>

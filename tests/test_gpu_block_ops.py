@@ -219,6 +219,15 @@ def test_boundary_gradient_sizes(eng, cols):
                    accumulate=k % 2 == 1)
 
 
+@pytest.mark.parametrize("cols", [4100, 8196, 8197, 12288, 12289, 16380])
+@pytest.mark.parametrize("boundary", [False, True])
+def test_gradient_of_wide_rows(eng, cols, boundary):
+    """Rows of every shape past 4,096 columns, of every type, in more rows than one launch takes."""
+    rng = np.random.default_rng(cols + boundary)
+    for k, (dt, st, dxt) in enumerate(BOUNDARY_TYPES if boundary else [(d, s, s) for s, d in NORM_TYPES]):
+        check_grad(eng, rng, 517 + k, cols, dt, st, dxt, boundary, accumulate=k % 2 == 0, pad=k % 3)
+
+
 @pytest.mark.parametrize("rows", [64, 257, 512, 513, 1000, 4097, 12288])
 def test_gradient_many_rows(eng, rows):
     """Rows past every workgroup's first ones; the sums over them, and each alone."""
