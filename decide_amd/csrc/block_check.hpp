@@ -74,7 +74,7 @@ inline Refusal arrays(const char *op, const Array *v, int n) {
       continue;
     }
     if ((uintptr_t)a.p % a.es) return {DN_INVALID_ARG, said(op) + a.name + " is not aligned to its elements"};
-    if (a.ld < 0 || (a.rows > 1 && a.ld < a.cols))
+    if (a.rows > 1 && a.ld < a.cols)
       return {DN_INVALID_ARG, said(op) + "the row stride of " + a.name + " is less than its columns"};
     if (a.rows > 1 && a.ld > ((int64_t)1 << 56) / a.rows)
       return {DN_INVALID_ARG, said(op) + "the row stride of " + a.name + " passes the address range"};

@@ -48,6 +48,12 @@ int run(dn_ctx *c, const char *op, Check check, Launch launch) {
   }
 }
 
+// Floats of workspace for sizes that the checks pass; 0 for others, which they refuse.
+int64_t work_floats(int64_t rows, int cols) {
+  const bool taken = rows >= 0 && rows <= blockchk::kMaxRows && cols >= 1 && cols <= kNormMaxCols;
+  return taken ? norm_grad_work(rows, cols) : 0;
+}
+
 }  // namespace
 
 extern "C" {
@@ -97,7 +103,7 @@ int dn_layer_norm_backward_device(dn_ctx *c, int dy_type, int x_type, int64_t ro
   a.accumulate = accumulate ? 1 : 0;
   a.work = (float *)d_work;
   return run(c, "layer_norm_backward",
-             [&] { return blockchk::norm_grad(dy_type, x_type, a, norm_grad_work(rows, cols), work_bytes); },
+             [&] { return blockchk::norm_grad(dy_type, x_type, a, work_floats(rows, cols), work_bytes); },
              [&] { return launch_norm_grad(dy_type, x_type, a, c->stream); });
 }
 
@@ -171,7 +177,7 @@ int dn_dropout_add_norm_backward_device(dn_ctx *c, int dy_type, int stream_type,
   return run(c, "dropout_add_norm_backward",
              [&] {
                return blockchk::boundary_grad(dy_type, stream_type, dx_type, p, seed, offset, &a,
-                                              norm_grad_work(rows, cols), work_bytes);
+                                              work_floats(rows, cols), work_bytes);
              },
              [&] { return launch_boundary_grad(dy_type, stream_type, dx_type, a, c->stream); });
 }

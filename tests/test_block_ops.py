@@ -128,6 +128,18 @@ def test_null_misaligned_and_narrow_arrays(checks, op):
 
 
 @pytest.mark.parametrize("op", OPS)
+def test_a_single_row_has_any_stride(checks, op):
+    for ld in (0, 1, 23, -1, -(1 << 63), (1 << 63) - 1):
+        strides = {n: ld for n in dir(NormCall) if n.startswith("ld")}
+        assert call(checks, op, rows=1, **strides)[0] == OK
+        # A gradient's h is an input: two inputs may overlap.
+        inputs = ("h",) if op.endswith("grad") else ()
+        for o in [n for n in USES[op] if hasattr(NormCall, "ld" + n) and n in OUT and n not in inputs]:
+            other = next(n for n in USES[op] if n != o)
+            assert call(checks, op, rows=1, **strides, **{o: (NAMES.index(other) + 1 << 20) + 4})[0] == INVALID
+
+
+@pytest.mark.parametrize("op", OPS)
 def test_sizes(checks, op):
     assert call(checks, op, rows=-1)[0] == INVALID
     assert call(checks, op, rows=1 << 31)[0] == UNSUPPORTED

@@ -719,5 +719,13 @@ def test_refusals_reach_the_caller(eng):
         eng.dropout_device("fp32", "fp32", 4, 64, x.at, 64, None, 0, 1.5, 1, 2, y.at, 64)
     with pytest.raises(InvalidArgument, match="x is NULL"):
         eng.dropout_device("fp32", "fp32", 4, 64, None, 64, None, 0, 0.5, 1, 2, y.at, 64)
+    for rows, cols in ((2 ** 63 - 1, 64), (2 ** 31, 64), (600, 2 ** 31 - 1), (2 ** 63 - 1, 2 ** 31 - 1)):
+        for dw in (None, y.at):
+            with pytest.raises(Unsupported, match="at most"):
+                eng.layer_norm_backward_device("fp32", "fp32", rows, cols, x.at, 64, x.at, 64, None, x.at, x.at, y.at,
+                                               64, dw)
+    for rows, cols in ((-1, 64), (600, -1), (-2 ** 63, -2 ** 31)):
+        with pytest.raises(InvalidArgument, match="rows or columns"):
+            eng.layer_norm_backward_device("fp32", "fp32", rows, cols, x.at, 64, x.at, 64, None, x.at, x.at, y.at, 64)
     torch.cuda.synchronize()
     assert bool((y.buf == GUARD).all())
