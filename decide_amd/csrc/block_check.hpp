@@ -55,8 +55,9 @@ inline bool apart(const Array &a, const Array &b) {
   auto lo = [](const Array &x) { return (uintptr_t)x.p; };
   auto span = [](const Array &x) { return (uint64_t)(((x.rows - 1) * x.ld + x.cols) * x.es); };
   if (lo(a) + span(a) <= lo(b) || lo(b) + span(b) <= lo(a)) return true;
+  if (a.rows < 2 || b.rows < 2) return false;  // a single row's stride is any number
   const int64_t sa = a.ld * a.es, sb = b.ld * b.es;
-  if (sa != sb || a.rows < 2 || b.rows < 2) return false;
+  if (sa != sb) return false;
   // b's first byte within a's row, modulo the stride.
   const int64_t d = lo(b) >= lo(a) ? (int64_t)((lo(b) - lo(a)) % (uint64_t)sa)
                                    : (sa - (int64_t)((lo(a) - lo(b)) % (uint64_t)sa)) % sa;
