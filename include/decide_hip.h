@@ -408,9 +408,10 @@ int dn_set_trainable(dn_ctx *ctx, int train_from, int train_emb);
  * stored: element (token t of the batch, column c) after layer l's attention
  * (site 0) or MLP (site 1) has row t, column c, this seed and the offset
  * forward * 2 * layers + 2 * l + site, where `forward` is `step` in the next
- * dn_forward_train and one more in each after it while p > 0. dn_backward
- * regenerates the masks of its forward, whatever was set since. A resumed run
- * passes the number of forwards already made. The default is p = 0 (no
+ * dn_forward_train and one more in each after it while p > 0; a call without
+ * tokens or one that is refused does not count. dn_backward regenerates the
+ * masks of its forward, whatever was set since. A resumed run passes the
+ * number of forwards that counted. The default is p = 0 (no
  * dropout, the kernels without it). Needs dn_enable_training;
  * dn_set_config clears it. No counterpart in the reference, which trains
  * without dropout. */

@@ -73,3 +73,23 @@ def test_micro_batches_add_up(prec):
             assert np.all(np.abs(both - (a + b)) <= 1100 * 2.0 ** -24 * size.max()), n
             if n.endswith(("mlp_norm.weight", "attn_norm.weight", "Wo.weight", "Wqkv.weight")):
                 assert np.linalg.norm(a - b) > 0.05 * np.linalg.norm(a), n
+
+
+def test_a_call_without_tokens_does_not_count():
+    """Nor does a refused one: the masks that follow are those of the step that was set."""
+    from decide_amd import InvalidArgument, native
+
+    cfg = small_cfg(2)
+    none = np.zeros(1, np.int32), np.zeros(1, np.float32)
+    w, batch = weights_for(cfg), make(cfg, 673)
+    with open_train(cfg, w, "fp32") as eng:
+        eng.set_dropout(0.3, 5, 4)
+        want = eng.forward(batch)
+        eng.set_dropout(0.3, 5, 4)
+        assert native.lib.dn_forward_train(eng.handle, 0, *[none[0].ctypes.data] * 6,
+                                           none[1].ctypes.data, 1) == native.DN_OK
+        bad = train_batch(cfg.vocab, 399, specs=BATCHES[673])
+        bad[0].ids[3] = cfg.vocab + 5
+        with pytest.raises(InvalidArgument):
+            eng.forward(bad)
+        assert np.array_equal(eng.forward(batch), want)
