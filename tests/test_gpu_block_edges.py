@@ -1,13 +1,49 @@
-"""The training-block operators at the edges of their ranges."""
+"""The training-block operators at the edges of their ranges: rows far from zero
+against bounds that only a corrected mean keeps, and rows whose padded columns
+would leave fp32's range."""
 import numpy as np
 import pytest
 import torch
 
 import block_reference as ref
-from test_gpu_block_ops import BOUNDARY_TYPES, NORM_TYPES, Matrix, eng, f64, ptr, vec, within  # noqa: F401
-
+from block_bounds import far_rows, two_pass_bounds
+from test_gpu_block_ops import (BOUNDARY_TYPES, EPS, NORM_TYPES, Matrix, eng, f64, ptr, vec,  # noqa: F401
+                                within)
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("cols", [3, 7, 64, 100, 768, 1000, 1021, 2900, 4099, 8190, 16384])
+def test_norm_of_rows_far_from_zero(eng, cols):
+    """y, mean and rstd of rows up to 100,000 times their spread from zero, and of constant rows, as two passes
+    give them (test_block_bounds.py: without the correction of the mean they are off by more)."""
+    rng = np.random.default_rng(cols)
+    rows = far_rows(rng, cols)
+    w, b = vec(1 + 0.2 * rng.standard_normal(cols)), vec(0.3 * rng.standard_normal(cols))
+    n = len(rows)
+    for xt, yt in NORM_TYPES:
+        for weights in ((None, None), (w, b)):
+            x, y = Matrix(n, cols, xt, torch.from_numpy(rows).clamp(-6e4, 6e4)), Matrix(n, cols, yt)
+            mean, rstd = torch.empty(n, device="cuda"), torch.empty(n, device="cuda")
+            eng.layer_norm_device(xt, yt, n, cols, x.at, cols, ptr(weights[0]), ptr(weights[1]), EPS, y.at, cols,
+                                  ptr(mean), ptr(rstd))
+            args = x.f64(), f64(weights[0]), f64(weights[1]), EPS
+            want = ref.norm(*args)
+            for got, wanted, bound, what in zip((y.f64(), f64(mean), f64(rstd)), want,
+                                                two_pass_bounds(*args, *want, yt), ("y", "mean", "rstd")):
+                within(got, wanted, bound, (what, cols, xt, yt))
+    # The boundary, h being those rows: res + 0.
+    x, res = Matrix(n, cols, "fp32", torch.zeros(n, cols)), Matrix(n, cols, "fp32", torch.from_numpy(rows))
+    h, y = Matrix(n, cols, "fp32"), Matrix(n, cols, "fp32")
+    mean, rstd = torch.empty(n, device="cuda"), torch.empty(n, device="cuda")
+    eng.dropout_add_norm_device("fp32", "fp32", "fp32", n, cols, x.at, cols, res.at, cols, 0.1, 1, 2, ptr(w), ptr(b), EPS,
+                                h.at, cols, y.at, cols, ptr(mean), ptr(rstd))
+    assert torch.equal(h.view, res.view)
+    args = h.f64(), f64(w), f64(b), EPS
+    want = ref.norm(*args)
+    for got, wanted, bound, what in zip((y.f64(), f64(mean), f64(rstd)), want, two_pass_bounds(*args, *want, "fp32"),
+                                        ("y", "mean", "rstd")):
+        within(got, wanted, bound, ("boundary", what, cols))
 
 
 @pytest.mark.parametrize("rows", [6, 520])
