@@ -1,14 +1,14 @@
 """The training-block operators at the edges of their ranges: rows far from zero
-against bounds that only a corrected mean keeps, and rows whose padded columns
-would leave fp32's range."""
+against bounds that only a corrected mean keeps, rows whose padded columns
+would leave fp32's range, and dropout of more elements than one launch takes."""
 import numpy as np
 import pytest
 import torch
 
 import block_reference as ref
 from block_bounds import far_rows, two_pass_bounds
-from test_gpu_block_ops import (BOUNDARY_TYPES, EPS, NORM_TYPES, Matrix, eng, f64, ptr, vec,  # noqa: F401
-                                within)
+from test_gpu_block_ops import (BOUNDARY_TYPES, EPS, GUARD, NORM_TYPES, TYPES, Matrix, eng, f64, ptr,  # noqa: F401
+                                vec, within)
 
 pytestmark = pytest.mark.gpu
 
@@ -87,3 +87,34 @@ def test_gradient_of_large_constant_rows(eng, cols, rows):
             within(dx.f64(), wanted, np.where(keep, e + ref.rounding(np.abs(wanted) + e, dxt), 0.0), ("dx", *what))
         assert not gw.any() and torch.equal(dw, torch.zeros_like(dw)), what
         within(db, gb, eb + ref.U * np.abs(gb), ("db", *what))
+
+
+def test_dropout_writes_nothing_past_a_long_row(eng):
+    """A row of more than 2^31 columns, two launches, the last vector a part of one: its last columns are right and
+    what stands behind them stays."""
+    long = 2 ** 31 + 21
+    buf = torch.full((long + 32,), GUARD, dtype=torch.bfloat16, device="cuda")
+    buf[:long] = 1.0
+    eng.dropout_device("bf16", "bf16", 1, long, ptr(buf), long, None, 0, 0.5, 3, 4, ptr(buf), long)
+    for c0 in (0, 2 ** 31 - 64, long - 64):
+        c = np.arange(c0, c0 + 64)
+        keep, scale = ref.keep_scale(np.zeros(1, np.int64), c, 0.5, 3, 4)
+        assert np.array_equal(buf[c0: c0 + 64].float().cpu().numpy(), (keep[0] * scale).astype(np.float32)), c0
+    assert bool((buf[long:] == GUARD).all())
+
+
+@pytest.mark.parametrize("xt,yt", [("bf16", "bf16"), ("bf16", "fp32")])
+def test_dropout_of_more_elements_than_a_launch_takes(eng, xt, yt):
+    """2^28 blocks of eight columns a launch: the second one starts inside a row."""
+    cols, per = 8197, 1025
+    split = 2 ** 28 // per
+    rows = split + 5
+    x = torch.zeros(rows, cols, dtype=TYPES[xt], device="cuda")
+    y = torch.full((rows * cols + 32,), GUARD, dtype=TYPES[yt], device="cuda")
+    at = [0, 1, split - 1, split, split + 1, rows - 1]
+    x[at] = torch.from_numpy(np.random.default_rng(5).standard_normal((6, cols))).to(TYPES[xt]).cuda()
+    eng.dropout_device(xt, yt, rows, cols, ptr(x), cols, None, 0, 0.25, 6, 7, ptr(y), cols)
+    want = ref.drop(f64(x[at]), ref.keep_scale(np.array(at), cols, 0.25, 6, 7))
+    got = y[:rows * cols].view(rows, cols)
+    within(got[at], want, 2 * ref.U * np.abs(want) + ref.rounding(np.abs(want) * (1 + 2 * ref.U), yt), (xt, yt))
+    assert bool((y[rows * cols:] == GUARD).all()) and not bool(got[2:split - 1].any())
