@@ -478,10 +478,13 @@ int dn_set_adam_step(dn_ctx *ctx, int step);
  * fp32. An output may be an input's very array (the same address, stride and
  * element size); any other overlap with an output is refused (DN_INVALID_ARG),
  * as are NULL, misaligned or too-narrow arrays. rows may be 0. Norms take 1 to
- * 16,384 columns (DN_UNSUPPORTED beyond). A row with an infinity or a NaN
- * gives NaN in that row and, through dw and db, in their sums. No counterpart
- * in the reference, whose model has no dropout and whose LayerNorm
- * (internal/nn/ops.go:63-138) runs inside it. */
+ * 16,384 columns (DN_UNSUPPORTED beyond). A row of a norm's input with an
+ * infinity or a NaN gives NaN in that row; in a gradient dy's and the input's
+ * also reach the sums of their columns, and dh's its own elements alone. Rows
+ * of elements up to 1e17 in magnitude stay in fp32's range at every width;
+ * beyond, a row whose sum, or sum of squared differences, passes 3.4e38 has no
+ * defined y and statistics. No counterpart in the reference, whose model has
+ * no dropout and whose LayerNorm (internal/nn/ops.go:63-138) runs inside it. */
 
 /* y = (x - mean) * rstd * w + b over each row, mean = sum x / cols, rstd =
  * 1 / sqrt(sum (x - mean)^2 / cols + eps), eps > 0. d_w NULL: 1, d_b NULL: 0.

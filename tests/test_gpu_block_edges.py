@@ -1,6 +1,7 @@
-"""The training-block operators at the edges of their ranges: rows far from zero
-against bounds that only a corrected mean keeps, rows whose padded columns
-would leave fp32's range, and dropout of more elements than one launch takes."""
+"""The training-block operators at the edges of their ranges: rows far from
+zero against bounds that only a corrected mean keeps, rows whose padded columns
+would leave fp32's range, the largest values the norms take, and dropout of
+more elements than one launch takes."""
 import numpy as np
 import pytest
 import torch
@@ -87,6 +88,23 @@ def test_gradient_of_large_constant_rows(eng, cols, rows):
             within(dx.f64(), wanted, np.where(keep, e + ref.rounding(np.abs(wanted) + e, dxt), 0.0), ("dx", *what))
         assert not gw.any() and torch.equal(dw, torch.zeros_like(dw)), what
         within(db, gb, eb + ref.U * np.abs(gb), ("db", *what))
+
+
+@pytest.mark.parametrize("cols", [5, 768, 4099, 16384])
+def test_largest_values(eng, cols):
+    """Elements of up to 1e17 in magnitude stay in fp32's range at every width."""
+    rng = np.random.default_rng(cols)
+    rows = 1e17 * rng.uniform(-1, 1, (6, cols))
+    rows[1] = np.where(rng.random(cols) < 0.5, 1e17, -1e17)
+    rows[2] = 1e17 - 1e10 * rng.random(cols)
+    for xt, yt in (("fp32", "fp32"), ("fp32", "bf16"), ("bf16", "bf16")):
+        x, y = Matrix(6, cols, xt, torch.from_numpy(rows)), Matrix(6, cols, yt)
+        mean, rstd = torch.empty(6, device="cuda"), torch.empty(6, device="cuda")
+        eng.layer_norm_device(xt, yt, 6, cols, x.at, cols, None, None, EPS, y.at, cols, ptr(mean), ptr(rstd))
+        want = ref.norm(x.f64(), None, None, EPS)
+        bounds = two_pass_bounds(x.f64(), None, None, EPS, *want, yt)
+        for got, wanted, bound, what in zip((y.f64(), f64(mean), f64(rstd)), want, bounds, ("y", "mean", "rstd")):
+            within(got, wanted, bound, (what, cols, xt, yt))
 
 
 def test_dropout_writes_nothing_past_a_long_row(eng):
