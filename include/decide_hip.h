@@ -512,9 +512,9 @@ int dn_layer_norm_backward_device(dn_ctx *ctx, int dy_type, int x_type, int64_t 
                                   int accumulate, void *d_work, int64_t work_bytes);
 
 /* y = dropout(x), or res + dropout(x) with d_res (of y's type). With t =
- * round(65536 * p), an element is kept, and multiplied by 65536 / (65536 - t),
- * where its 16 random bits are at least t, and is 0 otherwise, whatever it
- * was. The mask is never stored: the bits are a function of (seed, offset,
+ * 65536 * p to the nearest integer (ties to even), an element is kept, and
+ * multiplied by 65536 / (65536 - t), where its 16 random bits are at least t,
+ * and is 0 otherwise, whatever it was. The mask is never stored: the bits are a function of (seed, offset,
  * row, column) alone, the halves of Philox4x32-10 (Salmon et al., SC'11) with
  * the seed as its key and (column / 8, row, offset low, offset high) as its
  * counter: column 8k + 2j + i takes half i (0 low, 1 high) of word j. Calls
