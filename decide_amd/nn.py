@@ -161,6 +161,13 @@ def row_tokens(batch: Seq[Sequence]) -> np.ndarray:
     return np.array(out, np.int32)
 
 
+def _within_c(*sizes: int, cols: Optional[int] = None) -> list:
+    """Sizes as the C ABI's int64 holds them, and cols last as its int does: what passes either becomes its
+    largest or smallest value, which the library's own checks judge."""
+    out = [max(min(v, 2 ** 63 - 1), -2 ** 63) for v in sizes]
+    return out if cols is None else out + [max(min(cols, 2 ** 31 - 1), -2 ** 31)]
+
+
 class Engine:
     """A device-resident model: the counterpart of gpunn.Model as returned by
     train.NewInferer (internal/train/engine.go:152-167). forward(batch) has
@@ -326,19 +333,23 @@ class Engine:
     # The training-block operators (include/decide_hip.h). Arguments named d_*
     # are raw device addresses, strides are in elements; asynchronous on the
     # engine's stream. They use the engine's device and stream, not its model.
+    # Seeds and offsets are taken modulo 2^64. Sizes that pass their C type,
+    # whose upper bits ctypes would drop, go to the library as that type's ends.
 
     def layer_norm_device(self, x_type: str, y_type: str, rows: int, cols: int, d_x: int, ldx: int,
                           d_w: Optional[int], d_b: Optional[int], eps: float, d_y: int, ldy: int,
                           d_mean: Optional[int] = None, d_rstd: Optional[int] = None) -> None:
         """dn_layer_norm_device: y = (x - mean) * rstd * w + b per row; mean and rstd kept when given."""
         P = native.PRECISIONS
+        if (rows | ldx | ldy) >> 63 or cols >> 31:
+            rows, ldx, ldy, cols = _within_c(rows, ldx, ldy, cols=cols)
         check(lib.dn_layer_norm_device(self._h, P[x_type], P[y_type], rows, cols, d_x, ldx, d_w, d_b, eps, d_y, ldy,
                                        d_mean, d_rstd), self._h)
 
     @staticmethod
     def norm_backward_workspace(rows: int, cols: int) -> int:
         """dn_norm_backward_workspace: bytes of d_work for the two norm backward calls."""
-        n = lib.dn_norm_backward_workspace(rows, cols)
+        n = lib.dn_norm_backward_workspace(*_within_c(rows, cols=cols))
         if n < 0:
             raise ValueError(f"norm_backward_workspace: {rows} rows of {cols} columns")
         return n
@@ -350,6 +361,8 @@ class Engine:
                                    work_bytes: int = 0) -> None:
         """dn_layer_norm_backward_device: dx, and dw / db (= or +=) when given."""
         P = native.PRECISIONS
+        if (rows | lddy | ldx | lddx) >> 63 or cols >> 31:
+            rows, lddy, ldx, lddx, cols = _within_c(rows, lddy, ldx, lddx, cols=cols)
         check(lib.dn_layer_norm_backward_device(self._h, P[dy_type], P[x_type], rows, cols, d_dy, lddy, d_x, ldx, d_w,
                                                 d_mean, d_rstd, d_dx, lddx, d_dw, d_db, bool(accumulate), d_work,
                                                 work_bytes), self._h)
@@ -359,6 +372,8 @@ class Engine:
                        ldy: int) -> None:
         """dn_dropout_device: y = [res +] dropout(x); its own gradient with the same p, seed and offset."""
         P = native.PRECISIONS
+        if (rows | cols | ldx | ldres | ldy) >> 63:
+            rows, cols, ldx, ldres, ldy = _within_c(rows, cols, ldx, ldres, ldy)
         check(lib.dn_dropout_device(self._h, P[x_type], P[y_type], rows, cols, d_x, ldx, d_res, ldres, p, seed, offset,
                                     d_y, ldy), self._h)
 
@@ -368,6 +383,8 @@ class Engine:
                                 ldy: int, d_mean: Optional[int] = None, d_rstd: Optional[int] = None) -> None:
         """dn_dropout_add_norm_device: h = res + dropout(x), y = LayerNorm(h)."""
         P = native.PRECISIONS
+        if (rows | ldx | ldres | ldh | ldy) >> 63 or cols >> 31:
+            rows, ldx, ldres, ldh, ldy, cols = _within_c(rows, ldx, ldres, ldh, ldy, cols=cols)
         check(lib.dn_dropout_add_norm_device(self._h, P[x_type], P[stream_type], P[y_type], rows, cols, d_x, ldx,
                                              d_res, ldres, p, seed, offset, d_w, d_b, eps, d_h, ldh, d_y, ldy, d_mean,
                                              d_rstd), self._h)
@@ -381,6 +398,8 @@ class Engine:
                                          work_bytes: int = 0) -> None:
         """dn_dropout_add_norm_backward_device: dres = dh + LayerNorm'(dy), dx = dropout'(dres), dw, db."""
         P = native.PRECISIONS
+        if (rows | lddy | lddh | ldh | lddres | lddx) >> 63 or cols >> 31:
+            rows, lddy, lddh, ldh, lddres, lddx, cols = _within_c(rows, lddy, lddh, ldh, lddres, lddx, cols=cols)
         check(lib.dn_dropout_add_norm_backward_device(self._h, P[dy_type], P[stream_type], P[dx_type], rows, cols,
                                                       d_dy, lddy, d_dh, lddh, d_h, ldh, p, seed, offset, d_w, d_mean,
                                                       d_rstd, d_dres, lddres, d_dx, lddx, d_dw, d_db, bool(accumulate),
