@@ -128,7 +128,8 @@ def prepare(case, seed):
         return v
 
     kind = case["kind"]
-    st = {"case": case, "rows": rows, "cols": cols, "ld": ld}
+    # The stream that made the inputs; the calls on them go there too.
+    st = {"case": case, "rows": rows, "cols": cols, "ld": ld, "stream": torch.cuda.current_stream().cuda_stream}
     if "p" in case:
         bits = torch.randint(0, 2 ** 31, (4,), generator=gen, device="cuda").tolist()
         st["seed"], st["offset"] = bits[0] << 32 | bits[1] << 1, bits[2] << 20 | bits[3] & 0xFFFFF
@@ -235,13 +236,15 @@ def _plain(st):
 _kept = {}
 
 
-def _engine():
+def _engine(stream):
     if "engine" not in _kept:
         from decide_amd.nn import Config, Engine
 
         cfg = Config(hidden=256, intermediate=384, heads=4, layers=1, vocab=8, layer_types=["full_attention"])
         _kept["engine"] = Engine(cfg, None, precision="fp32")
-        _kept["engine"].set_stream(torch.cuda.current_stream().cuda_stream)
+    if _kept.get("stream") != stream:
+        _kept["engine"].set_stream(stream)
+        _kept["stream"] = stream
     return _kept["engine"]
 
 
@@ -261,7 +264,7 @@ def _sums(st, eng):
 
 
 def _own(st):
-    case, kind, eng = st["case"], st["case"]["kind"], _engine()
+    case, kind, eng = st["case"], st["case"]["kind"], _engine(st["stream"])
     rows, cols, ld = st["rows"], st["cols"], st["ld"]
     if kind == "norm":
         eng.layer_norm_device(case["stream"], case["out"], rows, cols, _at(st["x"]), ld, _at(st["w"]), _at(st["b"]),
