@@ -238,10 +238,11 @@ int backward_impl(dn_ctx *c, const float *dlogits) {
   // dact only when the GeGLU backward cannot run in the GEMM's epilogue.
   if (!gemm_epi_ok(prec, EPI_GEGLU_BWD, T)) HIPCHK(c, "hipMalloc", ensure(tr.dact, 4 * (size_t)T * I));
   HIPCHK(c, "hipMalloc", ensure(tr.dctx, es * TH));
-  HIPCHK(c, "hipMalloc", ensure(tr.dop_out, es * TH));
-  HIPCHK(c, "hipMalloc", ensure(tr.dop_h1, es * TH));
   const bool drop = tr.used.p > 0.0f;
-  if (drop) {
+  if (!drop) {
+    HIPCHK(c, "hipMalloc", ensure(tr.dop_out, es * TH));
+    HIPCHK(c, "hipMalloc", ensure(tr.dop_h1, es * TH));
+  } else {
     for (int q = 0; q < 2; q++) {
       HIPCHK(c, "hipMalloc", ensure(tr.drop_out[q], es * TH));
       HIPCHK(c, "hipMalloc", ensure(tr.drop_h1[q], es * TH));

@@ -93,3 +93,20 @@ def test_a_call_without_tokens_does_not_count():
         with pytest.raises(InvalidArgument):
             eng.forward(bad)
         assert np.array_equal(eng.forward(batch), want)
+
+
+def test_training_without_dropout_after_training_with_it():
+    """A backward pass without dropout in a context whose first ones had it: the bits of one that never had."""
+    cfg = small_cfg()
+    w, batch = weights_for(cfg), make(cfg, 673)
+    dl = dlogits(batch)
+    got = []
+    for ps in ((0.0,), (0.2, 0.0)):
+        with open_train(cfg, w, "bf16") as eng:
+            for p in ps:
+                eng.set_dropout(p, 3)
+                eng.zero_grad()
+                logits = eng.forward(batch)
+                eng.backward(dl)
+            got.append([logits] + [eng.download(n, "grad") for n in w])
+    assert all(np.array_equal(a, b) for a, b in zip(*got))
