@@ -131,16 +131,12 @@ __global__ __launch_bounds__(Shape::MAXT) void norm_grad_kernel(NormGradArgs a, 
 #pragma unroll
       for (int i = 0; i < VEC; i++) w[i] = 1.0f;
       if (weight) load<float, VEC>(weight, c, cols, w);
-      unpack<S, VEC>(h[j], cols - c, xh[j]);
+      // Columns past the row hold dy = 0 and xh = 0 (of h = mean: mean * rstd may be infinite where no column's xh is).
+      unpack<S, VEC>(h[j], cols - c, xh[j], mean);
       unpack<D, VEC>(dy[j], cols - c, g[j]);
 #pragma unroll
-      for (int i = 0; i < VEC; i++) xh[j][i] = (xh[j][i] - mean) * rstd;
-      // Columns past the row hold dy = 0, and xh = 0: mean * rstd may be infinite where no column's xh is.
-      if (cols - c < VEC)
-#pragma unroll
-        for (int i = 0; i < VEC; i++) xh[j][i] = i < cols - c ? xh[j][i] : 0.0f;
-#pragma unroll
       for (int i = 0; i < VEC; i++) {
+        xh[j][i] = (xh[j][i] - mean) * rstd;
         sw[j][i] += g[j][i] * xh[j][i];
         sb[j][i] += g[j][i];
         g[j][i] *= w[i];

@@ -146,9 +146,9 @@ __device__ __forceinline__ Raw<T, VEC> fetch(const T *row, int c, int cols) {
   return r;
 }
 
-// The vector's elements as floats, zeros past the row. n: columns from c on.
+// The vector's elements as floats, `past` past the row. n: columns from c on.
 template <class T, int VEC>
-__device__ __forceinline__ void unpack(const Raw<T, VEC> &r, int n, float (&v)[VEC]) {
+__device__ __forceinline__ void unpack(const Raw<T, VEC> &r, int n, float (&v)[VEC], float past = 0.0f) {
 #pragma unroll
   for (int j = 0; j < VEC; j++) v[j] = r.at(j);
   if (n < VEC) {
@@ -156,7 +156,7 @@ __device__ __forceinline__ void unpack(const Raw<T, VEC> &r, int n, float (&v)[V
 #pragma unroll
     for (int step = VEC; step > 0; step >>= 1)
 #pragma unroll
-      for (int j = 0; j < VEC; j++) v[j] = by & step ? (j + step < VEC ? v[j + step] : 0.0f) : v[j];
+      for (int j = 0; j < VEC; j++) v[j] = by & step ? (j + step < VEC ? v[j + step] : past) : v[j];
   }
 }
 
