@@ -5,22 +5,32 @@
 
 namespace {
 
+// Calls of at most this many rows sum each column over all of them in
+// workgroups beside those of the rows: one launch (of ~3.5 us on the host)
+// instead of two, for a second read of dy and h from the caches. Norm gradient,
+// bf16 dy and fp32 stream, one launch and two, us (arrays in the cache):
+//   columns        768          2,304          4,096          8,192
+//   256 rows    5.2   7.8     5.2   8.9      7.1  11.2      7.5  16.0
+//   512         5.2   8.0     9.1  11.5     15.1  15.8     14.3  16.3
+//   640         5.9   7.8    10.6  12.8     19.6  15.5     18.3  17.8
+//   1,024      11.4   8.3    17.1  14.6     29.0  15.7     27.6  21.9
+// One number for all widths: up to 2,304 columns one launch still wins at 768
+// rows; the boundary's gradient at 4,096 columns wants two from about 450 on
+// (512 rows of fp32: 19.9 and 15.7).
+constexpr int64_t kSmallRows = 512;
+// Columns of such a workgroup: few, so that many threads share the rows, or 32
+// where the columns alone make enough workgroups and narrow reads cost more
+// (the same gradient at 512 rows, 8 and 32: 768 columns 5.2 and 11.6 us, 2,304
+// 9.2 and 12.5, 4,000 13.6 and 14.1, 4,096 14.8 and 13.9, 6,144 22.3 and 13.5,
+// 8,192 30.4 and 14.3; all in bf16 4,000 12.4 and 13.3, 4,104 12.8 and 18.8,
+// 6,144 19.3 and 17.9).
+__host__ __device__ constexpr int slab_cols(int cols) { return cols <= 4096 ? 8 : 32; }
+
 // Workgroups of the gradient of many rows, each with partial sums of its own
 // that cost a slice of the workspace to write and to read again: up to three
 // per CU while they make 16 waves together (12,288 x 768: 768 workgroups 37.4
 // us, 512 39.0, 1,024 38.2), one past 4,096 columns (4,096 x 8,192: 256
 // workgroups 75 us, 512 82).
-// Calls of at most this many rows sum each column over all of them in
-// workgroups beside those of the rows: one launch (of ~3.5 us on the host)
-// instead of two, for a second read of dy and h from the caches. One launch and
-// two: 256 x 768 8.3 and 10.8 us, 512 x 768 8.3 and 10.9, 768 x 768 11.0 and 10.8,
-// 1,024 x 768 13.7 and 10.9; 512 x 8,192 14.7 and 16.4, 1,024 x 8,192 27.7 and 26.9.
-constexpr int64_t kSmallRows = 512;
-// Columns of such a workgroup: few, so that many threads share the rows (512 x
-// 768: 8 columns 8.3 us, 16 8.6, 32 11.7), or 32 where the columns alone make
-// enough workgroups and narrow reads cost more (512 x 8,192: 30, 20 and 14.7).
-__host__ __device__ constexpr int slab_cols(int cols) { return cols <= 4096 ? 8 : 32; }
-
 int row_parts(int64_t rows, int cols, int rows_per_group, int threads) {
   const int most = 256 * (cols > 4096 ? 1 : std::clamp(1024 / threads, 1, 3));
   return (int)std::min<int64_t>(most, (rows + rows_per_group - 1) / rows_per_group);
@@ -76,8 +86,8 @@ __device__ __forceinline__ void column_sums(const NormGradArgs &a, int slab) {
 // workgroup's sums go to its slice of the workspace. SMALL: the
 // workgroups past `groups` sum the columns instead.
 //
-// HBM-bound: 12,288 x 768 (dy bf16, stream fp32) 18.7 us, with dropout's gradient
-// 30.2, both 5 TB/s; the sums that follow (norm_join_kernel) 4 to 5 us more. The
+// HBM-bound: 12,288 x 768 (dy bf16, stream fp32) 20 us, with dropout's gradient
+// 31, both 4.7 to 4.9 TB/s; the sums that follow (norm_join_kernel) 4 to 5 us more. The
 // rows of a workgroup come from a loop, since its sums live in registers; three
 // to four waves per SIMD cover the loop's wait for its stores.
 template <class D, class S, class X, bool BOUNDARY, bool SMALL, class Shape>

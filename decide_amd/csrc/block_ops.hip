@@ -18,7 +18,7 @@ constexpr int kGrid = 1 << 20;
 // per thread group and no loop over rows: loads and stores share one counter
 // (vmcnt), so that a loop's next row waits for this row's stores (32,768 x 768
 // with a row prefetched in a loop 58 us, without a loop 29.5, 5.1 TB/s, the
-// rate of a large copy; 12,288 rows with dropout 45 and 23.5, 4.8 TB/s). The
+// rate of a large copy; 12,288 rows with dropout 45 and 23.9, 4.7 TB/s). The
 // weights are read after the sums, not held: at most 64 registers, eight waves
 // per SIMD. 768 x 64 rows: 3.1 us on the GPU, 4.6 a call.
 template <class X, class S, class Y, bool BOUNDARY, class Shape>
