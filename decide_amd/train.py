@@ -40,7 +40,7 @@ class TrainEngine(Engine):
     def set_dropout(self, p: float, seed: int = 0, step: int = 0) -> None:
         """dn_set_dropout: dropout of every sub-layer's output in the training forwards that
         follow; step: the number of forwards already made with this seed (a resumed run), those of no
-        tokens left out."""
+        tokens left out. Ranks that train together pass a seed each."""
         check(lib.dn_set_dropout(self._h, float(p), int(seed), int(step)), self._h)
 
     def infer(self, batch: Seq[Sequence]) -> np.ndarray:

@@ -411,8 +411,12 @@ int dn_set_trainable(dn_ctx *ctx, int train_from, int train_emb);
  * dn_forward_train and one more in each after it while p > 0; a call without
  * tokens or one that is refused does not count. dn_backward regenerates the
  * masks of its forward, whatever was set since. A resumed run passes the
- * number of forwards that counted. The default is p = 0 (no
- * dropout, the kernels without it). Needs dn_enable_training;
+ * number of forwards that counted. A token's row is its place in this
+ * context's batch, so contexts that train together on different batches (one
+ * per GPU) need a seed each, or they drop the same elements. Nothing else is
+ * dropped: not the embeddings, the attention's probabilities or the MLP's
+ * activations before Wo (where some recipes have it instead). The default is
+ * p = 0 (no dropout, the kernels without it). Needs dn_enable_training;
  * dn_set_config clears it. No counterpart in the reference, which trains
  * without dropout. */
 int dn_set_dropout(dn_ctx *ctx, float p, uint64_t seed, uint64_t step);
