@@ -42,8 +42,8 @@ __host__ __device__ constexpr int sum_stride(int cols) { return (cols + 3) / 4 *
 
 // dw and db of COLS columns over all rows (of few), by one workgroup: its
 // threads share the rows, eight loaded at a time, and their sums are added in
-// order.
-template <class D, class S, int COLS>
+// order. RMS: there is no mean.
+template <class D, class S, int COLS, bool RMS>
 __device__ __forceinline__ void column_sums(const NormGradArgs &a, int slab) {
   constexpr int BATCH = 8;
   __shared__ float lds[2][1024 / COLS][COLS + 1];
@@ -57,7 +57,7 @@ __device__ __forceinline__ void column_sums(const NormGradArgs &a, int slab) {
       const int64_t row = min(r + j * step, rows - 1);
       dy[j] = (float)((const D *)a.dy)[row * a.lddy + at];
       h[j] = (float)((const S *)a.h)[row * a.ldh + at];
-      mean[j] = a.mean[row];
+      mean[j] = RMS ? 0.0f : a.mean[row];
       rstd[j] = a.rstd[row];
     }
 #pragma unroll
@@ -84,18 +84,19 @@ __device__ __forceinline__ void column_sums(const NormGradArgs &a, int slab) {
 // dropout's gradient of it (the forward's mask and scale), from the unrounded
 // sum. Each thread adds dy xh and dy of its columns over its rows; a
 // workgroup's sums go to its slice of the workspace. SMALL: the
-// workgroups past `groups` sum the columns instead.
+// workgroups past `groups` sum the columns instead. RMS: the norm has no mean
+// (xh = h rstd, no mean(g)) and no bias, and dx may be null.
 //
 // HBM-bound: 12,288 x 768 (dy bf16, stream fp32) 20 us, with dropout's gradient
 // 31, both 4.7 to 4.9 TB/s; the sums that follow (norm_join_kernel) 4 to 5 us more. The
 // rows of a workgroup come from a loop, since its sums live in registers; three
 // to four waves per SIMD cover the loop's wait for its stores.
-template <class D, class S, class X, bool BOUNDARY, bool SMALL, class Shape>
+template <class D, class S, class X, bool BOUNDARY, bool SMALL, class Shape, bool RMS>
 __global__ __launch_bounds__(Shape::MAXT) void norm_grad_kernel(NormGradArgs a, int groups) {
   if constexpr (SMALL)
     if ((int)blockIdx.x >= groups) {
       const int slab = blockIdx.x - groups;
-      return slab_cols(a.cols) == 8 ? column_sums<D, S, 8>(a, slab) : column_sums<D, S, 32>(a, slab);
+      return slab_cols(a.cols) == 8 ? column_sums<D, S, 8, RMS>(a, slab) : column_sums<D, S, 32, RMS>(a, slab);
     }
   constexpr int VEC = Shape::VEC, LPR = Shape::LPR, VPT = Shape::VPT;
   constexpr bool WAVES = LPR == 0;
@@ -131,7 +132,7 @@ __global__ __launch_bounds__(Shape::MAXT) void norm_grad_kernel(NormGradArgs a, 
           dh[j] = fetch<S, VEC>((const S *)a.dh + row * a.lddh, VEC * (lane + j * lpr), cols);
     };
     if constexpr (BOUNDARY && !LATE) fetch_dh();
-    const float mean = a.mean[row], rstd = a.rstd[row];
+    const float mean = RMS ? 0.0f : a.mean[row], rstd = a.rstd[row];
     float g[VPT][VEC], xh[VPT][VEC];
     float s[2] = {0.0f, 0.0f};
 #pragma unroll
@@ -156,7 +157,7 @@ __global__ __launch_bounds__(Shape::MAXT) void norm_grad_kernel(NormGradArgs a, 
     }
     row_sum<LPR>(s, slots[turn]);
     if constexpr (LATE) fetch_dh();
-    const float c1 = mul_rounded(s[0], inv), c2 = mul_rounded(s[1], inv);
+    const float c1 = RMS ? 0.0f : mul_rounded(s[0], inv), c2 = mul_rounded(s[1], inv);
 #pragma unroll
     for (int j = 0; j < VPT; j++) {
       const int c = VEC * (lane + j * lpr);
@@ -171,7 +172,11 @@ __global__ __launch_bounds__(Shape::MAXT) void norm_grad_kernel(NormGradArgs a, 
         }
       store<S, VEC>((S *)a.dres + row * a.lddres, c, cols, g[j]);
     }
-    if constexpr (BOUNDARY) {
+    if constexpr (RMS) {
+      if (a.dx)
+#pragma unroll
+        for (int j = 0; j < VPT; j++) store<X, VEC>((X *)a.dx + row * a.lddx, VEC * (lane + j * lpr), cols, g[j]);
+    } else if constexpr (BOUNDARY) {
       Columns<WAVES, VPT, VEC>::drop(a.mask, (uint32_t)row, lane, lpr, cols, g);
 #pragma unroll
       for (int j = 0; j < VPT; j++) {
@@ -284,7 +289,7 @@ hipError_t with_grad_shape(int cols, F f) {
                       RowShape<4, 0, 3, 1024>, RowShape<4, 0, 4, 1024>>(cols, f);
 }
 
-template <class D, class S, class X, bool BOUNDARY>
+template <class D, class S, class X, bool BOUNDARY, bool RMS = false>
 hipError_t grad_launch(const NormGradArgs &args, hipStream_t s) {
   return with_grad_shape<vec_of<D, S, X>>(args.cols, [&](auto shape) {
     using Shape = decltype(shape);
@@ -296,7 +301,7 @@ hipError_t grad_launch(const NormGradArgs &args, hipStream_t s) {
       const int slabs = sums ? (a.cols + slab - 1) / slab : 0;
       auto run = [&](int grid, int row_groups) {
         if (grid > 0)
-          hipLaunchKernelGGL((norm_grad_kernel<D, S, X, BOUNDARY, true, Shape>), dim3(grid), dim3(threads), 0, s, a,
+          hipLaunchKernelGGL((norm_grad_kernel<D, S, X, BOUNDARY, true, Shape, RMS>), dim3(grid), dim3(threads), 0, s, a,
                              row_groups);
         return hipGetLastError();
       };
@@ -308,7 +313,7 @@ hipError_t grad_launch(const NormGradArgs &args, hipStream_t s) {
     }
     const int parts = row_parts(a.rows, a.cols, Shape::ROWS, threads);
     if (!sums) a.work = nullptr;
-    hipLaunchKernelGGL((norm_grad_kernel<D, S, X, BOUNDARY, false, Shape>), dim3(parts), dim3(threads), 0, s, a, parts);
+    hipLaunchKernelGGL((norm_grad_kernel<D, S, X, BOUNDARY, false, Shape, RMS>), dim3(parts), dim3(threads), 0, s, a, parts);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || !sums) return e;
     hipLaunchKernelGGL(norm_join_kernel, dim3((a.cols + 31) / 32, a.db ? 2 : 1), dim3(1024), 0, s, a, parts);
@@ -324,11 +329,12 @@ hipError_t norm_grad_pick(int dy_type, int x_type, const NormGradArgs &a, hipStr
   return grad_launch<T, T, T, false>(a, s);
 }
 
-template <class T>
+template <class T, bool RMS>
 hipError_t boundary_grad_pick(int dy_type, int stream_type, int dx_type, const NormGradArgs &a, hipStream_t s) {
-  if (stream_type != PREC_F32) return grad_launch<T, T, T, true>(a, s);
-  if (dx_type == PREC_F32) return grad_launch<float, float, float, true>(a, s);
-  return dy_type == PREC_F32 ? grad_launch<float, float, T, true>(a, s) : grad_launch<T, float, T, true>(a, s);
+  if (stream_type != PREC_F32) return grad_launch<T, T, T, true, RMS>(a, s);
+  if (dx_type == PREC_F32) return grad_launch<float, float, float, true, RMS>(a, s);
+  return dy_type == PREC_F32 ? grad_launch<float, float, T, true, RMS>(a, s)
+                             : grad_launch<T, float, T, true, RMS>(a, s);
 }
 
 }  // namespace
@@ -352,6 +358,11 @@ hipError_t launch_norm_grad(int dy_type, int x_type, const NormGradArgs &a, hipS
 }
 
 hipError_t launch_boundary_grad(int dy_type, int stream_type, int dx_type, const NormGradArgs &a, hipStream_t s) {
-  return dx_type == PREC_F16 ? boundary_grad_pick<f16>(dy_type, stream_type, dx_type, a, s)
-                             : boundary_grad_pick<bf16>(dy_type, stream_type, dx_type, a, s);
+  return dx_type == PREC_F16 ? boundary_grad_pick<f16, false>(dy_type, stream_type, dx_type, a, s)
+                             : boundary_grad_pick<bf16, false>(dy_type, stream_type, dx_type, a, s);
+}
+
+hipError_t launch_rms_grad(int dy_type, int stream_type, int dx_type, const NormGradArgs &a, hipStream_t s) {
+  return dx_type == PREC_F16 ? boundary_grad_pick<f16, true>(dy_type, stream_type, dx_type, a, s)
+                             : boundary_grad_pick<bf16, true>(dy_type, stream_type, dx_type, a, s);
 }

@@ -4,49 +4,11 @@
 // is allocated, copied or waited for, so the calls can be captured into a graph.
 #include <hip/hip_runtime.h>
 
-#include <exception>
-#include <string>
-
 #include "block_check.hpp"
 #include "block_ops.hpp"
-#include "ctx.hpp"
-
-using namespace dnh;
+#include "device_call.hpp"
 
 namespace {
-
-// The context's device for the duration of a call; the caller's current one
-// comes back after it.
-struct OnDevice {
-  int before = -1;
-  hipError_t err;
-  explicit OnDevice(int device) {
-    err = hipGetDevice(&before);
-    if (err == hipSuccess && before != device) err = hipSetDevice(device);
-    if (before == device) before = -1;
-  }
-  ~OnDevice() {
-    if (before >= 0) (void)hipSetDevice(before);
-  }
-};
-
-// check() gives a blockchk::Refusal, launch() a hipError_t. No C++ exception
-// (an allocation that fails while a message is built) leaves the C entry point.
-template <class Check, class Launch>
-int run(dn_ctx *c, const char *op, Check check, Launch launch) {
-  if (!c) return DN_INVALID_ARG;
-  try {
-    c->err.clear();
-    const blockchk::Refusal r = check();
-    if (r.code) return fail(c, r.code, r.msg);
-    const OnDevice on(c->device);
-    HIPCHK(c, "hipSetDevice", on.err);
-    HIPCHK(c, op, launch());
-    return DN_OK;
-  } catch (const std::exception &) {
-    return DN_OUT_OF_MEMORY;
-  }
-}
 
 // Floats of workspace for sizes that the checks pass; 0 for others, which they refuse.
 int64_t work_floats(int64_t rows, int cols) {
@@ -73,7 +35,7 @@ int dn_layer_norm_device(dn_ctx *c, int x_type, int y_type, int64_t rows, int co
   a.ldy = ldy;
   a.mean = d_mean;
   a.rstd = d_rstd;
-  return run(c, "layer_norm", [&] { return blockchk::norm(x_type, y_type, a); },
+  return device_call(c, "layer_norm", [&] { return blockchk::norm(x_type, y_type, a); },
              [&] { return launch_norm(x_type, y_type, a, c->stream); });
 }
 
@@ -102,7 +64,7 @@ int dn_layer_norm_backward_device(dn_ctx *c, int dy_type, int x_type, int64_t ro
   a.db = d_db;
   a.accumulate = accumulate ? 1 : 0;
   a.work = (float *)d_work;
-  return run(c, "layer_norm_backward",
+  return device_call(c, "layer_norm_backward",
              [&] { return blockchk::norm_grad(dy_type, x_type, a, work_floats(rows, cols), work_bytes); },
              [&] { return launch_norm_grad(dy_type, x_type, a, c->stream); });
 }
@@ -119,7 +81,7 @@ int dn_dropout_device(dn_ctx *c, int x_type, int y_type, int64_t rows, int64_t c
   a.ldres = ldres;
   a.y = d_y;
   a.ldy = ldy;
-  return run(c, "dropout", [&] { return blockchk::dropout(x_type, y_type, p, seed, offset, &a); },
+  return device_call(c, "dropout", [&] { return blockchk::dropout(x_type, y_type, p, seed, offset, &a); },
              [&] { return launch_dropout(x_type, y_type, a, c->stream); });
 }
 
@@ -143,7 +105,7 @@ int dn_dropout_add_norm_device(dn_ctx *c, int x_type, int stream_type, int y_typ
   a.ldy = ldy;
   a.mean = d_mean;
   a.rstd = d_rstd;
-  return run(c, "dropout_add_norm",
+  return device_call(c, "dropout_add_norm",
              [&] { return blockchk::boundary(x_type, stream_type, y_type, p, seed, offset, &a); },
              [&] { return launch_boundary(x_type, stream_type, y_type, a, c->stream); });
 }
@@ -174,7 +136,7 @@ int dn_dropout_add_norm_backward_device(dn_ctx *c, int dy_type, int stream_type,
   a.db = d_db;
   a.accumulate = accumulate ? 1 : 0;
   a.work = (float *)d_work;
-  return run(c, "dropout_add_norm_backward",
+  return device_call(c, "dropout_add_norm_backward",
              [&] {
                return blockchk::boundary_grad(dy_type, stream_type, dx_type, p, seed, offset, &a,
                                               work_floats(rows, cols), work_bytes);

@@ -15,6 +15,8 @@ hipError_t launch_norm(int x_type, int y_type, const NormArgs &a, hipStream_t s)
 hipError_t launch_boundary(int x_type, int stream_type, int y_type, const NormArgs &a, hipStream_t s);
 hipError_t launch_norm_grad(int dy_type, int x_type, const NormGradArgs &a, hipStream_t s);
 hipError_t launch_boundary_grad(int dy_type, int stream_type, int dx_type, const NormGradArgs &a, hipStream_t s);
+// The RMS norm's gradient: no mean, bias or mask; dx may be null.
+hipError_t launch_rms_grad(int dy_type, int stream_type, int dx_type, const NormGradArgs &a, hipStream_t s);
 int64_t norm_grad_work(int64_t rows, int cols);
 hipError_t launch_dropout(int x_type, int y_type, const DropArgs &a, hipStream_t s);
 

@@ -18,6 +18,8 @@ LIB_PATH = os.environ.get("DECIDE_HIP_LIBRARY") or os.path.join(HERE, "libdecide
 DN_OK, DN_NO_GPU, DN_INVALID_ARG, DN_OUT_OF_MEMORY, DN_DEVICE_ERROR, DN_UNSUPPORTED = range(6)
 DN_PRECISION_FP32, DN_PRECISION_BF16, DN_PRECISION_FP16 = 0, 1, 2
 PRECISIONS = {"fp32": DN_PRECISION_FP32, "bf16": DN_PRECISION_BF16, "fp16": DN_PRECISION_FP16}
+DN_FP8_E4M3, DN_FP8_E5M2 = 3, 4
+FP8_TYPES = {"e4m3": DN_FP8_E4M3, "e5m2": DN_FP8_E5M2}
 DN_STATE_WEIGHT, DN_STATE_GRAD, DN_STATE_M, DN_STATE_V = range(4)
 
 
@@ -104,6 +106,15 @@ _SIGS = {
                                     _i64, _vp, _i64, _vp, _vp], _i),
     "dn_dropout_add_norm_backward_device": ([_vp, _i, _i, _i, _i64, _i, _vp, _i64, _vp, _i64, _vp, _i64, _f, _u64, _u64,
                                              _vp, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _i, _vp, _i64], _i),
+    "dn_add_rms_norm_device": ([_vp, _i, _i, _i, _i, _i64, _i, _vp, _i64, _vp, _i64, _vp, _f, _vp, _i64, _vp, _i64, _vp,
+                                _i64, _vp, _i64, _vp], _i),
+    "dn_add_rms_norm_backward_device": ([_vp, _i, _i, _i, _i64, _i, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _i64,
+                                         _vp, _i64, _vp, _i, _vp, _i64], _i),
+    "dn_quantize_blocks_device": ([_vp, _i, _i, _i64, _i64, _i, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64],
+                                  _i),
+    "dn_gemm_fp8_workspace": ([_i64, _i64, _i64], _i64),
+    "dn_gemm_fp8_device": ([_vp, _i, _i, _i, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _i, _vp, _i64, _vp, _i64,
+                            _i, _vp, _i64], _i),
     "dn_tokenizer_parse": ([_vp, _c.c_int64, _c.POINTER(_vp)], _i),
     "dn_tokenizer_free": ([_vp], None),
     "dn_tokenizer_special_ids": ([_vp, _vp, _vp, _vp, _vp], _i),

@@ -405,6 +405,68 @@ class Engine:
                                                       d_rstd, d_dres, lddres, d_dx, lddx, d_dw, d_db, bool(accumulate),
                                                       d_work, work_bytes), self._h)
 
+    # The 8-bit projection operators (include/decide_hip.h): conventions as
+    # above. 8-bit types are "e4m3" and "e5m2"; the scale of block of columns b
+    # and row r is at d_scale[b * ldscale + r].
+
+    def add_rms_norm_device(self, x_type: str, stream_type: str, y_type: str, q_type: str, rows: int, cols: int,
+                            d_x: int, ldx: int, d_res: Optional[int], ldres: int, d_w: Optional[int], eps: float,
+                            d_h: Optional[int], ldh: int, d_y: Optional[int], ldy: int, d_q: Optional[int], ldq: int,
+                            d_scale: Optional[int], ldscale: int, d_rstd: Optional[int] = None) -> None:
+        """dn_add_rms_norm_device: h = res + x, y = RMSNorm(h), q and scale = y in 8 bits."""
+        P, Q = native.PRECISIONS, native.FP8_TYPES
+        if (rows | ldx | ldres | ldh | ldy | ldq | ldscale) >> 63 or cols >> 31:
+            rows, ldx, ldres, ldh, ldy, ldq, ldscale, cols = _within_c(rows, ldx, ldres, ldh, ldy, ldq, ldscale,
+                                                                       cols=cols)
+        check(lib.dn_add_rms_norm_device(self._h, P[x_type], P[stream_type], P[y_type], Q[q_type], rows, cols, d_x, ldx,
+                                         d_res, ldres, d_w, eps, d_h, ldh, d_y, ldy, d_q, ldq, d_scale, ldscale,
+                                         d_rstd), self._h)
+
+    def add_rms_norm_backward_device(self, dy_type: str, stream_type: str, dx_type: str, rows: int, cols: int,
+                                     d_dy: int, lddy: int, d_dh: Optional[int], lddh: int, d_h: int, ldh: int,
+                                     d_w: Optional[int], d_rstd: int, d_dres: int, lddres: int, d_dx: Optional[int],
+                                     lddx: int, d_dw: Optional[int] = None, accumulate: bool = False,
+                                     d_work: Optional[int] = None, work_bytes: int = 0) -> None:
+        """dn_add_rms_norm_backward_device: dres = dx = dh + RMSNorm'(dy), dw; norm_backward_workspace bytes."""
+        P = native.PRECISIONS
+        if (rows | lddy | lddh | ldh | lddres | lddx) >> 63 or cols >> 31:
+            rows, lddy, lddh, ldh, lddres, lddx, cols = _within_c(rows, lddy, lddh, ldh, lddres, lddx, cols=cols)
+        check(lib.dn_add_rms_norm_backward_device(self._h, P[dy_type], P[stream_type], P[dx_type], rows, cols, d_dy,
+                                                  lddy, d_dh, lddh, d_h, ldh, d_w, d_rstd, d_dres, lddres, d_dx, lddx,
+                                                  d_dw, bool(accumulate), d_work, work_bytes), self._h)
+
+    def quantize_blocks_device(self, x_type: str, q_type: str, rows: int, cols: int, block_rows: int, d_x: int,
+                               ldx: int, d_q: Optional[int], ldq: int, d_scale: Optional[int], ldscale: int,
+                               d_qt: Optional[int] = None, ldqt: int = 0, d_scalet: Optional[int] = None,
+                               ldscalet: int = 0) -> None:
+        """dn_quantize_blocks_device: x in 8 bits with a scale a block, and / or its transpose."""
+        if (rows | cols | ldx | ldq | ldscale | ldqt | ldscalet) >> 63 or block_rows >> 31:
+            rows, cols, ldx, ldq, ldscale, ldqt, ldscalet, block_rows = _within_c(rows, cols, ldx, ldq, ldscale, ldqt,
+                                                                                  ldscalet, cols=block_rows)
+        check(lib.dn_quantize_blocks_device(self._h, native.PRECISIONS[x_type], native.FP8_TYPES[q_type], rows, cols,
+                                            block_rows, d_x, ldx, d_q, ldq, d_scale, ldscale, d_qt, ldqt, d_scalet,
+                                            ldscalet), self._h)
+
+    @staticmethod
+    def gemm_fp8_workspace(M: int, N: int, K: int) -> int:
+        """dn_gemm_fp8_workspace: bytes of d_work for gemm_fp8_device."""
+        n = lib.dn_gemm_fp8_workspace(*_within_c(M, N, K))
+        if n < 0:
+            raise ValueError(f"gemm_fp8_workspace: {M} x {N} x {K}")
+        return n
+
+    def gemm_fp8_device(self, a_type: str, b_type: str, c_type: str, M: int, N: int, K: int, d_A: int, lda: int,
+                        d_sa: int, ldsa: int, d_B: int, ldb: int, b_rows: int, d_sb: int, ldsb: int, d_C: int,
+                        ldc: int, accumulate: bool = False, d_work: Optional[int] = None,
+                        work_bytes: int = 0) -> None:
+        """dn_gemm_fp8_device: C = [C +] A . B^T of 8-bit arrays, B's scales of b_rows x 128 blocks."""
+        Q = native.FP8_TYPES
+        if (M | N | K | lda | ldsa | ldb | ldsb | ldc) >> 63 or b_rows >> 31:
+            M, N, K, lda, ldsa, ldb, ldsb, ldc, b_rows = _within_c(M, N, K, lda, ldsa, ldb, ldsb, ldc, cols=b_rows)
+        check(lib.dn_gemm_fp8_device(self._h, Q[a_type], Q[b_type], native.PRECISIONS[c_type], M, N, K, d_A, lda, d_sa,
+                                     ldsa, d_B, ldb, b_rows, d_sb, ldsb, d_C, ldc, bool(accumulate), d_work,
+                                     work_bytes), self._h)
+
 
 def open_engine(cfg: Config, weights, precision="bf16", device=0) -> Engine:
     return Engine(cfg, weights, precision=precision, device=device)

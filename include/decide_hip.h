@@ -44,6 +44,9 @@ enum {
 
 enum { DN_PRECISION_FP32 = 0, DN_PRECISION_BF16 = 1, DN_PRECISION_FP16 = 2 };
 
+/* 8-bit types (OCP FP8) of the operators that say so; no precision of a model. */
+enum { DN_FP8_E4M3 = 3, DN_FP8_E5M2 = 4 };
+
 typedef struct dn_ctx dn_ctx;
 
 /* ABI version of the loaded library (DN_ABI_VERSION). */
@@ -550,6 +553,79 @@ int dn_dropout_add_norm_backward_device(dn_ctx *ctx, int dy_type, int stream_typ
                                         const float *d_w, const float *d_mean, const float *d_rstd, void *d_dres,
                                         int64_t lddres, void *d_dx, int64_t lddx, float *d_dw, float *d_db,
                                         int accumulate, void *d_work, int64_t work_bytes);
+
+/* ---- 8-bit projection operators on device arrays --------------------------
+ * Products of 8-bit floating-point arrays with a scale for each block of 128
+ * along the summed axis, the RMS norm that writes their operand, and the
+ * quantiser that makes the others: the 8-bit neighbours of dn_gemm_device and
+ * of the operators above, whose conventions hold here too (open context,
+ * stream, capture, strides, alignment, refusals), with these additions.
+ * An 8-bit array is of type DN_FP8_E4M3 (largest value 448) or DN_FP8_E5M2
+ * (57344). Its scales are fp32: the element at (r, c) stands for value *
+ * scale, scale at d_scale[b * ldscale + r'] with b = c / 128 and r' = r (blocks
+ * of 1 x 128) or r / 128 (128 x 128): a block of columns after the other, each
+ * with the rows side by side; ldscale at least the number of r' (any value for
+ * a single block of columns). The last block of a row or column may be partial.
+ * A block with a as its largest magnitude (2^-100 at least) has scale = a /
+ * largest value, and its elements are v * (largest value / a) rounded to
+ * nearest, ties to even. A block with an infinity has an infinite scale (each
+ * of its elements stands for a NaN); a NaN stays in its own element.
+ * Products are fastest with A, B and their row strides aligned to 16 bytes; any
+ * alignment is right. No counterpart in the reference. */
+
+/* h = res + x, rounded to the stream's type as it is stored; y = h * rstd * w
+ * of that h, rstd = 1 / sqrt(sum h^2 / cols + eps); q and its scales (blocks of
+ * 1 x 128) from the unrounded y. d_res NULL: h = x, which is not stored again
+ * (d_h is ignored; stream_type is x_type). Either of d_y and d_q (with
+ * d_scale) may be NULL; y_type is ignored without d_y. d_w NULL: 1. d_rstd ([rows],
+ * for the backward pass) may be NULL. x, stream and y types as
+ * dn_dropout_add_norm_device's. A NaN in a row of h makes that row of y NaN; an
+ * infinity alone makes rstd 0, the row's finite elements 0 and its own NaN. Sums
+ * of squares past 3.4e38 count as infinite. */
+int dn_add_rms_norm_device(dn_ctx *ctx, int x_type, int stream_type, int y_type, int q_type, int64_t rows, int cols,
+                           const void *d_x, int64_t ldx, const void *d_res, int64_t ldres, const float *d_w, float eps,
+                           void *d_h, int64_t ldh, void *d_y, int64_t ldy, void *d_q, int64_t ldq, float *d_scale,
+                           int64_t ldscale, float *d_rstd);
+
+/* Its gradients, the rounding to 8 bits passed straight through: with xh = h *
+ * rstd and g = dy * w,
+ *   dres = dh + rstd * (g - xh * mean(g * xh)),  dw = sum over rows of dy * xh.
+ * dres is the gradient of x too: d_dx, which may be NULL, receives the
+ * unrounded dres in a type of its own. d_dh (the gradient that reaches h beside
+ * the norm) may be NULL. dw is added to what d_dw holds when accumulate is set;
+ * d_dw may be NULL. d_work: dn_norm_backward_workspace bytes, with d_dw. Types
+ * as dn_dropout_add_norm_backward_device's; dx_type is ignored without d_dx. */
+int dn_add_rms_norm_backward_device(dn_ctx *ctx, int dy_type, int stream_type, int dx_type, int64_t rows, int cols,
+                                    const void *d_dy, int64_t lddy, const void *d_dh, int64_t lddh, const void *d_h,
+                                    int64_t ldh, const float *d_w, const float *d_rstd, void *d_dres, int64_t lddres,
+                                    void *d_dx, int64_t lddx, float *d_dw, int accumulate, void *d_work,
+                                    int64_t work_bytes);
+
+/* x [rows x cols] (fp32, bf16 or fp16) as 8-bit values with scales: q and scale
+ * of x, qt [cols x rows] and scalet of its transpose, from one read of x;
+ * either pair may be NULL. block_rows 1: blocks of 1 x 128 of each (activations
+ * and gradients: q for the product over the columns, qt for a weight's
+ * gradient, whose sum is over the rows). 128: blocks of 128 x 128, the
+ * same ones for both (weights: q for the forward product, qt for the input's
+ * gradient). */
+int dn_quantize_blocks_device(dn_ctx *ctx, int x_type, int q_type, int64_t rows, int64_t cols, int block_rows,
+                              const void *d_x, int64_t ldx, void *d_q, int64_t ldq, float *d_scale, int64_t ldscale,
+                              void *d_qt, int64_t ldqt, float *d_scalet, int64_t ldscalet);
+
+/* Bytes of d_work for a product of these sizes (0: none is needed, d_work may
+ * be NULL); -1 for sizes it does not take. */
+int64_t dn_gemm_fp8_workspace(int64_t M, int64_t N, int64_t K);
+
+/* C [M x N] = A [M x K] . B [N x K]^T of 8-bit arrays, A with scales of 1 x 128
+ * blocks, B of b_rows x 128 (b_rows 1 or 128): the sum over a block is fp32,
+ * times both scales (their product has to be in fp32's range) and added to the
+ * others' in fp32, rounded once to C's type (DN_PRECISION_*). accumulate: added
+ * to what C holds (fp32 C only). The sums' order depends on the sizes and
+ * alignments alone: equal calls give equal bits. K may be 0. */
+int dn_gemm_fp8_device(dn_ctx *ctx, int a_type, int b_type, int c_type, int64_t M, int64_t N, int64_t K,
+                       const void *d_A, int64_t lda, const float *d_sa, int64_t ldsa, const void *d_B, int64_t ldb,
+                       int b_rows, const float *d_sb, int64_t ldsb, void *d_C, int64_t ldc, int accumulate,
+                       void *d_work, int64_t work_bytes);
 
 #ifdef __cplusplus
 }
