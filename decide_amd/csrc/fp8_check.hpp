@@ -12,6 +12,8 @@ inline bool known8(int t) { return t == DN_FP8_E4M3 || t == DN_FP8_E5M2; }
 // Rows, columns and depth of an 8-bit array: a tile's number and a place
 // inside a row fit 32 bits.
 constexpr int64_t kMaxFp8 = 0x7fffffff;
+// Columns of a product: a row of tiles is one launch.
+constexpr int64_t kMaxFp8Out = 1 << 26;
 
 inline Refusal rms(int x_type, int stream_type, int y_type, int q_type, const RmsArgs &a) {
   const char *op = "dn_add_rms_norm_device";
@@ -74,8 +76,8 @@ inline Refusal quantise(int x_type, int q_type, int block_rows, const QuantArgs 
 
 inline Refusal gemm_sizes(const char *op, int64_t M, int64_t N, int64_t K) {
   if (M < 0 || N < 0 || K < 0) return {DN_INVALID_ARG, said(op) + "a size is negative"};
-  if (M > kMaxFp8 || N > kMaxFp8 || K > kMaxFp8)
-    return {DN_UNSUPPORTED, said(op) + "M, N and K of at most 2147483647"};
+  if (M > kMaxFp8 || N > kMaxFp8Out || K > kMaxFp8)
+    return {DN_UNSUPPORTED, said(op) + "M and K of at most 2147483647, N of at most 67108864"};
   return {};
 }
 

@@ -93,8 +93,7 @@ int dn_quantize_blocks_device(dn_ctx *c, int x_type, int q_type, int64_t rows, i
 }
 
 int64_t dn_gemm_fp8_workspace(int64_t M, int64_t N, int64_t K) {
-  for (const int64_t n : {M, N, K})
-    if (n < 0 || n > blockchk::kMaxFp8) return -1;
+  if (M < 0 || M > blockchk::kMaxFp8 || N < 0 || N > blockchk::kMaxFp8Out || K < 0 || K > blockchk::kMaxFp8) return -1;
   return gemm_fp8_work(M, N, K) * (int64_t)sizeof(float);
 }
 

@@ -122,18 +122,25 @@ __global__ __launch_bounds__(Shape::MAXT) void rms_kernel(RmsArgs a, int64_t fir
 #pragma unroll
     for (int i = 0; i < VEC; i++) w[i] = 1.0f;
     if (a.w) load<float, VEC>(a.w, c, cols, w);
-    float most = kLeast;
+    float most = 0.0f;
 #pragma unroll
     for (int i = 0; i < VEC; i++) {
-      v[j][i] = v[j][i] * rstd * w[i];
+      v[j][i] *= w[i];
       most = fmaxf(most, fabsf(v[j][i]));
     }
-    if (a.y) store<Y, VEC>((Y *)a.y + row * a.ldy, c, cols, v[j]);
     if (a.q) {
+      // y / scale without y's own rounding: rstd, which all of a block shares,
+      // cancels, unless the block is zeros, tiny or not finite.
       most = lanes_max<LANES>(most);
-      const float top = largest(a.e5m2);
-      store8<VEC>((uint8_t *)a.q + row * a.ldq, c, cols, v[j], top / most, a.e5m2);
-      if (lane % LANES == 0 && c < cols) a.scale[c / kFp8Block * a.ldscale + row] = most / top;
+      const float top = largest(a.e5m2), of_y = most * rstd;
+      const bool plain = of_y >= kLeast && of_y < INFINITY;
+      store8<VEC>((uint8_t *)a.q + row * a.ldq, c, cols, v[j], plain ? top / most : rstd * (top / kLeast), a.e5m2);
+      if (lane % LANES == 0 && c < cols) a.scale[c / kFp8Block * a.ldscale + row] = (plain ? of_y : kLeast) / top;
+    }
+    if (a.y) {
+#pragma unroll
+      for (int i = 0; i < VEC; i++) v[j][i] *= rstd;
+      store<Y, VEC>((Y *)a.y + row * a.ldy, c, cols, v[j]);
     }
   }
 }

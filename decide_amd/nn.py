@@ -450,7 +450,9 @@ class Engine:
     @staticmethod
     def gemm_fp8_workspace(M: int, N: int, K: int) -> int:
         """dn_gemm_fp8_workspace: bytes of d_work for gemm_fp8_device."""
-        n = lib.dn_gemm_fp8_workspace(*_within_c(M, N, K))
+        if (M | N | K) >> 63:
+            M, N, K = _within_c(M, N, K)
+        n = lib.dn_gemm_fp8_workspace(M, N, K)
         if n < 0:
             raise ValueError(f"gemm_fp8_workspace: {M} x {N} x {K}")
         return n
