@@ -98,80 +98,6 @@ __device__ __forceinline__ void put8(T *row, int64_t n, int64_t N, float (&v)[8]
   }
 }
 
-// A tile of 128 x 128 outputs, four waves of 64 x 64. Rows of 128 bytes in LDS,
-// their 16-byte chunks swizzled so that 16 lanes read distinct banks.
-template <bool EXACT, bool E5A, bool E5B, bool SQUARE>
-__global__ __launch_bounds__(256) void gemm_fp8_kernel(Fp8GemmArgs g, int c_type, uint32_t tiles_n) {
-  __shared__ __attribute__((aligned(16))) uint8_t tile[256][128];
-  __shared__ __attribute__((aligned(16))) float scale[256];
-  const int64_t m0 = (int64_t)(blockIdx.x / tiles_n) * 128, n0 = (int64_t)(blockIdx.x % tiles_n) * 128;
-  const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, wm = wave / 2, wn = wave % 2, r16 = lane % 16, g4 = lane / 16;
-  const uint8_t *src[8];
-#pragma unroll
-  for (int i = 0; i < 8; i++) {
-    const int r = i * 32 + tid / 8;
-    src[i] = r < 128 ? (const uint8_t *)g.A + min(m0 + r, g.M - 1) * g.lda
-                     : (const uint8_t *)g.B + min(n0 + r - 128, g.N - 1) * g.ldb;
-  }
-  const int64_t nrow = min(n0 + tid - 128, g.N - 1);
-  const float *ssrc = tid < 128 ? g.sa + min(m0 + tid, g.M - 1) : g.sb + (SQUARE ? nrow / 128 : nrow);
-  const int64_t sld = tid < 128 ? g.ldsa : g.ldsb;
-  auto swz = [](int r) { return r < 128 ? (r >> 1) & 7 : (r >> 1 & 1) | (r >> 2 & 6); };
-  f32x4 acc[4][4];
-#pragma unroll
-  for (int i = 0; i < 4; i++)
-#pragma unroll
-    for (int j = 0; j < 4; j++) acc[i][j] = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int64_t k0 = 0; k0 < g.K; k0 += 128) {
-    uint4 v[8];
-#pragma unroll
-    for (int i = 0; i < 8; i++) v[i] = chunk_of(src[i], k0 + tid % 8 * 16, g.K);
-    const float sv = ssrc[k0 / 128 * sld];
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-      const int r = i * 32 + tid / 8;
-      *(uint4 *)&tile[r][(tid % 8 ^ swz(r)) * 16] = v[i];
-    }
-    scale[tid] = sv;
-    __syncthreads();
-    auto chunk = [&](int r, int half) { return *(const uint4 *)&tile[r][(g4 ^ swz(r) ^ 4 * half) * 16]; };
-    uint4 b[4][2];
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-      const int r = 128 + wn * 64 + 32 * (j >> 1) + 4 * (j & 1) + 8 * (r16 >> 2) + (r16 & 3);
-      b[j][0] = chunk(r, 0), b[j][1] = chunk(r, 1);
-    }
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const Operand<EXACT, E5A> a(chunk(wm * 64 + i * 16 + r16, 0), chunk(wm * 64 + i * 16 + r16, 1));
-      const float sa = scale[wm * 64 + i * 16 + r16], sab = sa * scale[128 + wn * 64];
-#pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const f32x4 p = mma_block(Operand<EXACT, E5B>(b[j][0], b[j][1]), a);
-        const float *sb = scale + 128 + wn * 64 + 32 * (j >> 1) + 4 * (j & 1) + 8 * g4;
-#pragma unroll
-        for (int e = 0; e < 4; e++) acc[i][j][e] = fmaf(p[e], SQUARE ? sab : sa * sb[e], acc[i][j][e]);
-      }
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < 4; i++) {
-    const int64_t m = m0 + wm * 64 + i * 16 + r16;
-    if (m >= g.M) continue;
-#pragma unroll
-    for (int j = 0; j < 2; j++) {
-      float v[8];
-#pragma unroll
-      for (int e = 0; e < 8; e++) v[e] = acc[i][2 * j + (e >> 2)][e & 3];
-      const int64_t n = n0 + wn * 64 + 32 * j + 8 * g4;
-      if (c_type == PREC_F32) put8((float *)g.C + m * g.ldc, n, g.N, v, g.accumulate);
-      else if (c_type == PREC_BF16) put8((bf16 *)g.C + m * g.ldc, n, g.N, v, false);
-      else put8((f16 *)g.C + m * g.ldc, n, g.N, v, false);
-    }
-  }
-}
-
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 // A buffer of `bytes` from `base` on, for loads that read nothing past its end (a
@@ -229,18 +155,33 @@ struct TileAt {
 // on the global side of the load so that 16 lanes read distinct banks. The
 // operands' rows start at multiples of 16 bytes; what a load reads past a row's
 // end is its padding or the next row (nothing past the array's last chunk), and
-// the last block's partial chunks are masked in registers.
+// the last block's is cleared in LDS before it is multiplied. RAGGED: rows of any
+// alignment, through registers, whose unaligned loads bound it (4,001 x 4,099 x
+// 8,200 410 us, aligned 160; 4,096 x 768 x 768 16 and 9).
 //
 // B is the instruction's first operand, its rows dealt to the tiles of a wave so
 // that a lane holds runs of eight consecutive columns of C: 16 bytes of a 16-bit
 // C straight from registers, four lanes side by side.
-template <bool EXACT, bool E5A, bool E5B, bool SQUARE, int BM, int BN, int WGM, int WGN, bool ONE_B>
+//
+// ONE_B: B has one slot, since a wave holds a block's B in registers before the
+// next one's is needed: two workgroups of 128 x 256 tiles fit a CU's LDS, each of
+// which computes while the other waits (32,768 x 2,304 x 768: 90 us; 256 x 256 by
+// eight waves with two slots 99, 128 x 128 104; 8,192 cubed 494, 496, 557).
+//
+// Bound by power: at 8,192 cubed (2.2 PFLOP/s; a library product without block
+// scales 2.7) the matrix cores are 55% busy at 1.84 GHz, LDS 25%, no bank
+// conflicts. At K = 768 the tiles without their stores take 63 us and the stores
+// alone 36, and neither staggered starts nor more loads in flight overlap them.
+// EXACT: the vector unit, which widens the operands, and the matrix cores share a
+// wave's issue: 60% and 45% busy (1.1 PFLOP/s at 8,192 cubed).
+template <bool EXACT, bool E5A, bool E5B, bool SQUARE, int BM, int BN, int WGM, int WGN, bool ONE_B, bool RAGGED>
 __global__ __launch_bounds__(64 * WGM * WGN, 2) void gemm_fp8_tile_kernel(Fp8GemmArgs g, int c_type, uint32_t tiles_m,
                                                                          uint32_t tiles_n, uint32_t each) {
   constexpr int NW = WGM * WGN, WM = BM / WGM, WN = BN / WGN, TM = WM / 16, TN = WN / 16;
   constexpr int LOADS_A = BM / (8 * NW), LOADS_B = BN / (8 * NW), LOADS_S = (BM + BN + 64 * NW - 1) / (64 * NW);
   static_assert(NW % 4 == 0 && LOADS_A * 8 * NW == BM && LOADS_B * 8 * NW == BN && WN == 64, "a wave's share of a stage");
   static_assert(!ONE_B || !EXACT, "the loop that keeps B in registers across blocks");
+  static_assert(!RAGGED || (!ONE_B && BM + BN == 64 * NW), "a thread brings one scale");
   constexpr int AT_B = 2 * BM * 128, AT_S = AT_B + (ONE_B ? 1 : 2) * BN * 128, SCALES = LOADS_S * 256 * NW;
   __shared__ __attribute__((aligned(1024))) char smem[AT_S + 2 * SCALES];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -279,6 +220,42 @@ __global__ __launch_bounds__(64 * WGM * WGN, 2) void gemm_fp8_tile_kernel(Fp8Gem
     step_s[i] = 4 * (uint32_t)ld;
     asm volatile("s_nop 4" : "+s"(from_a), "+s"(from_b), "+s"(from_s[i]));  // written by vector instructions, read by to_lds
   }
+  // RAGGED: through registers instead, a block ahead of their way into LDS.
+  uint4 held_a[RAGGED ? LOADS_A : 1], held_b[RAGGED ? LOADS_B : 1];
+  float held_s = 0.0f;
+  auto hold = [&](int n) __attribute__((always_inline)) {
+    if (n >= count) return;
+    const int64_t k = (int64_t)(kb0 + n) * 128;
+    auto each = [&](auto read) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < (RAGGED ? LOADS_A : 0); i++)
+        held_a[i] = read((const uint8_t *)g.A + min(m0 + lrow + i * 8 * NW, g.M - 1) * g.lda,
+                         k + ((lane & 7) ^ swz_a(lrow)) * 16);
+#pragma unroll
+      for (int i = 0; i < (RAGGED ? LOADS_B : 0); i++)
+        held_b[i] = read((const uint8_t *)g.B + min(n0 + lrow + i * 8 * NW, g.N - 1) * g.ldb,
+                         k + ((lane & 7) ^ swz_b(lrow)) * 16);
+    };
+    if (k + 128 <= g.K)
+      each([](const uint8_t *row, int64_t at) {
+        uint4 v;
+        __builtin_memcpy(&v, row + at, 16);
+        return v;
+      });
+    else
+      each([&](const uint8_t *row, int64_t at) { return chunk_of(row, at, g.K); });
+    const int64_t row = tid < BM ? min(m0 + tid, g.M - 1) : min(n0 + tid - BM, g.N - 1) / (SQUARE ? 128 : 1);
+    held_s = tid < BM ? g.sa[(kb0 + n) * g.ldsa + row] : g.sb[(kb0 + n) * g.ldsb + row];
+  };
+  auto let_go = [&](int slot) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < (RAGGED ? LOADS_A : 0); i++)
+      *(uint4 *)(slot_a(slot) + (wave + i * NW) * 1024 + lane * 16) = held_a[i];
+#pragma unroll
+    for (int i = 0; i < (RAGGED ? LOADS_B : 0); i++)
+      *(uint4 *)(slot_b(slot) + (wave + i * NW) * 1024 + lane * 16) = held_b[i];
+    ((float *)slot_s(slot))[tid] = held_s;
+  };
   auto at_block = [&](int n, uint32_t step) { return n < count ? n * step : 1u << 31; };  // n: from kb0 on
   auto issue_a = [&](int slot, int n) {
     const uint32_t k = at_block(n, 128);
@@ -358,27 +335,36 @@ __global__ __launch_bounds__(64 * WGM * WGN, 2) void gemm_fp8_tile_kernel(Fp8Gem
     }
   };
 
-  // A block's slots are read once it has landed for every wave, and written once every wave is done with them.
-  auto landed = [] {
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
+  // A block's slots are read once it has landed for every wave, and written once
+  // every wave is done with them: from here on block n + 1 is read, n + 2 sent for.
+  auto change_over = [&](int slot, int n) __attribute__((always_inline)) {
+    if constexpr (RAGGED) {
+      let_go(slot ^ 1);
+      __syncthreads();
+      hold(n + 2);
+    } else {
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      issue_a(slot, n + 2);
+      if constexpr (!ONE_B) issue_b(slot, n + 2);
+    }
   };
   auto done = [] {
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
   };
   int slot = 0;
-  issue_a(0, 0);
-  issue_b(0, 0);
-  landed();
-  issue_a(1, 1);
-  if constexpr (!ONE_B) issue_b(1, 1);
+  if constexpr (RAGGED) {
+    hold(0);
+  } else {
+    issue_a(0, 0);
+    issue_b(0, 0);
+  }
+  change_over(1, -1);
   if constexpr (EXACT) {
     for (int n = 0; n < whole; n++, slot ^= 1) {
       multiply(slot);
-      landed();
-      issue_a(slot, n + 2);
-      issue_b(slot, n + 2);
+      change_over(slot, n);
     }
   } else if (whole > 0) {
     // As multiply(), across the blocks: the slots change over at row TM - 2,
@@ -408,9 +394,7 @@ __global__ __launch_bounds__(64 * WGM * WGN, 2) void gemm_fp8_tile_kernel(Fp8Gem
           sb = scale_b(next);
         }
         if (i == TM - 2) {
-          landed();
-          issue_a(slot, n + 2);
-          if constexpr (!ONE_B) issue_b(slot, n + 2);
+          change_over(slot, n);
         }
 #pragma unroll
         for (int j = 0; j < TN; j++) {
@@ -719,13 +703,8 @@ hipError_t launch_gemm_fp8(int a_e5m2, int b_e5m2, int c_type, const Fp8GemmArgs
     };
     const Kind kind = kind_of(args.M, args.N, args.K);
     if (kind != Kind::Tile) return any_small(args, kind);
-    if (!aligned)
-      return rows(args, 128, 128, [&](const Fp8GemmArgs &a, uint32_t tm, uint32_t tn) {
-        hipLaunchKernelGGL((gemm_fp8_kernel<X, A, B, S>), dim3(tm * tn), dim3(256), 0, s, a, c_type, tn);
-        return hipGetLastError();
-      });
     if constexpr (!X && S)
-      if (tiles_of(args.M, 128) * tiles_of(args.N, 256) >= 512) {
+      if (aligned && tiles_of(args.M, 128) * tiles_of(args.N, 256) >= 512) {
         // A last column of tiles that is nearly empty and costs a round of the
         // CUs goes to the small kernel (4,001 x 4,099 x 8,200: 198 -> 160 us).
         auto rounds = [&](int64_t N) { return tiles_of(tiles_of(args.M, 128) * tiles_of(N, 256), 512); };
@@ -741,7 +720,7 @@ hipError_t launch_gemm_fp8(int a_e5m2, int b_e5m2, int c_type, const Fp8GemmArgs
           if (e != hipSuccess) return e;
         }
         return rows(a, 128, 256, [&](const Fp8GemmArgs &a, uint32_t tm, uint32_t tn) {
-          hipLaunchKernelGGL((gemm_fp8_tile_kernel<X, A, B, S, 128, 256, 1, 4, true>), dim3(tm * tn), dim3(256), 0, s, a,
+          hipLaunchKernelGGL((gemm_fp8_tile_kernel<X, A, B, S, 128, 256, 1, 4, true, false>), dim3(tm * tn), dim3(256), 0, s, a,
                              c_type, tm, tn, (uint32_t)blocks);
           return hipGetLastError();
         });
@@ -750,8 +729,9 @@ hipError_t launch_gemm_fp8(int a_e5m2, int b_e5m2, int c_type, const Fp8GemmArgs
     const uint32_t each = (uint32_t)tiles_of(blocks, split);
     const int parts = each ? (int)tiles_of(blocks, each) : 1;
     const hipError_t e = rows(args, 128, 128, [&](const Fp8GemmArgs &a, uint32_t tm, uint32_t tn) {
-      hipLaunchKernelGGL((gemm_fp8_tile_kernel<X, A, B, S, 128, 128, 2, 2, false>), dim3(tm * tn, parts), dim3(256), 0, s, a,
-                         c_type, tm, tn, each);
+      auto kernel = aligned ? gemm_fp8_tile_kernel<X, A, B, S, 128, 128, 2, 2, false, false>
+                            : gemm_fp8_tile_kernel<X, A, B, S, 128, 128, 2, 2, false, true>;
+      hipLaunchKernelGGL(kernel, dim3(tm * tn, parts), dim3(256), 0, s, a, c_type, tm, tn, each);
       return hipGetLastError();
     });
     if (parts == 1 || e != hipSuccess) return e;
