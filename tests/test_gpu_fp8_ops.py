@@ -403,6 +403,14 @@ def test_gemm_larger(eng, M, N, K):
     check_gemm(eng, rng, M, N, K, pad=1, lead=1)
 
 
+@pytest.mark.parametrize("M,N,K", [(32641, 385, 300), (16385, 1024, 256), (8065, 2051, 2060)])
+def test_gemm_many_tiles(eng, M, N, K):
+    """512 tiles of 128 x 256 and more: K ending inside a block, whole blocks, a last column of tiles of its own."""
+    rng = np.random.default_rng(N)
+    for k, types in enumerate(GEMM_TYPES if N < 1000 else GEMM_TYPES[:1]):
+        check_gemm(eng, rng, M, N, K, types, ("bf16", "fp16")[k % 2], pad=-K % 16 + 16 * (k % 2), c_pad=(0, 3, 8, 1)[k])
+
+
 def test_gemm_empty(eng):
     """No rows, no columns: nothing happens. No depth: zeros, or C as it was."""
     rng = np.random.default_rng(1)
