@@ -2,16 +2,12 @@
 //   C[m][n] = sum over blocks b of sa[b][m] sb[b][n] sum over k in b of A[m][k] B[n][k]
 // One MFMA (16 x 16 x 128) is one block's inner sum of 16 x 16 outputs; its
 // result is scaled and added to the fp32 sums in registers.
-#include <algorithm>
-
 #include "fp8_ops.hpp"
+#include "fp8_plan.hpp"
 
 namespace {
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
-
-// Most tiles of a launch (fewer than 2^32 threads).
-constexpr int64_t kGrid = 1 << 22;
 
 // One 16 x 16 x 128 product. Lane l feeds row l % 16 of each operand with 32 of
 // the block's elements, the same ones for both (which ones is free: the sum over
@@ -611,132 +607,47 @@ __global__ __launch_bounds__(256) void gemm_fp8_join_kernel(Fp8GemmArgs g, int p
 
 }  // namespace
 
-namespace {
-
-int64_t tiles_of(int64_t n, int each) { return (n + each - 1) / each; }
-
-// The kernel of a product of these sizes. Times in us on the GPU, bf16 C with
-// 128 x 128 scales unless said:
-//                          16 x 16  32 x 32  64 x 32  128 x 128  128 x 256
-//   1 x 8,192 x 8,192        14.0     13.6     17.2      37.8
-//   16 x 8,192 x 4,096       10.8      9.8     11.5      21.1
-//   64 x 8,192 x 4,096       33.2     22.2     16.8      22.4
-//   100 x 768 x 768           4.4      4.6      5.7       7.3
-//   200 x 768 x 2,304         9.6      7.9     10.0      13.9
-//   512 x 768 x 768           8.9      7.2      6.0       7.9
-//   512 x 2,304 x 768        21.8     14.4     14.2       8.3
-//   4,096 x 2,304 x 768                                  18.6       19.6
-//   12,288 x 768 x 2,304                                 33.9       34.3
-//   4,096 x 4,096 x 4,096                                75.1       67.4
-//   32,768 x 2,304 x 768                                 103.8      90.2
-// The small kernel as long as one round of the CUs holds its tiles (its waves
-// share K, so that past 64 rows a long K goes to tiles whose parts workgroups
-// share: 384 x 384 x 12,288 into fp32 27.0 and 18.5).
-enum class Kind { Small11, Small22, Small42, Tile };
-Kind kind_of(int64_t M, int64_t N, int64_t K) {
-  if (M > 64 && K > 64 * 128) return Kind::Tile;
-  if (tiles_of(M, 16) * tiles_of(N, 16) <= 384) return Kind::Small11;
-  if (tiles_of(M, 32) * tiles_of(N, 32) <= 256) return Kind::Small22;
-  if (M <= 64 || tiles_of(M, 64) * tiles_of(N, 32) <= 256) return Kind::Small42;
-  return Kind::Tile;
-}
-
-// Workgroups that share a 128 x 128 tile's blocks along K, by what they cost: a
-// block 0.65 us (EXACT 1.2), half as much again for two workgroups on a CU, and
-// the join 7 us (a launch) and the partial sums' bytes (2,304 x 768 x 12,288
-// into fp32: one 123 us, two 75, four 65; 512 x 4,096 x 4,096 into bf16: one 23,
-// two 25, four 28).
-int split_of(int64_t M, int64_t N, int64_t K, bool exact) {
-  if (kind_of(M, N, K) != Kind::Tile) return 1;
-  const int64_t tiles = tiles_of(M, 128) * tiles_of(N, 128), blocks = tiles_of(K, 128);
-  int best = 1;
-  double least = 0.0;
-  for (int split = 1; split <= 16 && split * tiles <= 512 && (split == 1 || split * 4 <= blocks); split++) {
-    const double each = (exact ? 1.2 : 0.65) * (split * tiles > 256 ? 1.5 : 1.0);
-    const double cost = tiles_of(blocks, split) * each + (split > 1 ? 7.0 + split * (double)M * N * 8 / 4.5e6 : 0.0);
-    if (split == 1 || cost < least) best = split, least = cost;
-  }
-  return best;
-}
-
-}  // namespace
-
-int64_t gemm_fp8_work(int64_t M, int64_t N, int64_t K) {
-  const int split = M && N ? std::max(split_of(M, N, K, false), split_of(M, N, K, true)) : 1;
-  return split > 1 ? split * M * N : 0;
-}
+int64_t gemm_fp8_work(int64_t M, int64_t N, int64_t K) { return fp8plan::work_of(M, N, K); }
 
 hipError_t launch_gemm_fp8(int a_e5m2, int b_e5m2, int c_type, const Fp8GemmArgs &args, hipStream_t s) {
-  // Rows of whole 16-byte chunks, and offsets that fit a buffer load's 31 bits.
-  const int64_t blocks = tiles_of(args.K, 128);
-  auto fits = [&](const void *p, int64_t ld, int64_t ld_scale) {
-    return (uintptr_t)p % 16 == 0 && ld % 16 == 0 && ld >= 0 && ld <= 1 << 23 &&
-           (blocks <= 1 || (ld_scale <= 1 << 28 && ld_scale * blocks < 1 << 29));
-  };
-  const bool aligned = args.K <= 1 << 23 && fits(args.A, args.lda, args.ldsa) && fits(args.B, args.ldb, args.ldsb);
+  using fp8plan::Kind;
+  using fp8plan::Launch;
+  const bool direct = fp8plan::direct((uintptr_t)args.A, args.lda, args.ldsa, args.K) &&
+                      fp8plan::direct((uintptr_t)args.B, args.ldb, args.ldsb, args.K);
   auto with = [&](auto ex, auto ea, auto eb, auto sq) -> hipError_t {
     constexpr bool X = decltype(ex)::value, A = decltype(ea)::value, B = decltype(eb)::value, S = decltype(sq)::value;
-    // Rows of tiles in launches of at most kGrid tiles.
-    auto rows = [&](Fp8GemmArgs a, int bm, int bn, auto launch) -> hipError_t {
-      const int64_t tn = tiles_of(a.N, bn), most = std::max<int64_t>(1, kGrid / tn) * bm;
-      const int es = c_type == PREC_F32 ? 4 : 2;
-      for (int64_t left = a.M; left > 0; left -= most) {
-        a.M = std::min(left, most);
-        const hipError_t e = launch(a, (uint32_t)tiles_of(a.M, bm), (uint32_t)tn);
-        if (e != hipSuccess) return e;
-        a.A = (const char *)a.A + most * a.lda;
-        a.sa += most;
-        a.C = (char *)a.C + most * a.ldc * es;
-      }
-      return hipSuccess;
-    };
-    auto small = [&](const Fp8GemmArgs &args, auto kernel, int bm, int bn) {
-      return rows(args, bm, bn, [&](const Fp8GemmArgs &a, uint32_t tm, uint32_t tn) {
+    int parts = 1;
+    auto launch = [&](const Launch &l) -> hipError_t {
+      Fp8GemmArgs a = args;
+      a.M = l.M;
+      a.N = l.N;
+      a.A = (const char *)args.A + l.m * args.lda;
+      a.sa = args.sa + l.m;
+      a.B = (const char *)args.B + l.n * args.ldb;
+      a.sb = args.sb + (S ? l.n / kFp8Block : l.n);
+      a.C = (char *)args.C + (l.m * args.ldc + l.n) * (c_type == PREC_F32 ? 4 : 2);
+      parts = l.parts;
+      const uint32_t tm = l.tiles_m, tn = l.tiles_n;
+      auto small = [&](auto kernel) {
         hipLaunchKernelGGL(kernel, dim3(tm * tn), dim3(64 * kSmallWaves), 0, s, a, c_type, tm, tn);
         return hipGetLastError();
-      });
+      };
+      auto tile = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3(tm * tn, parts), dim3(256), 0, s, a, c_type, tm, tn, l.each);
+        return hipGetLastError();
+      };
+      if (l.kind == Kind::Small11) return small(gemm_fp8_small_kernel<X, A, B, S, 1, 1, 3>);
+      if (l.kind == Kind::Small22) return small(gemm_fp8_small_kernel<X, A, B, S, 2, 2, 2>);
+      if (l.kind == Kind::Small42) return small(gemm_fp8_small_kernel<X, A, B, S, 4, 2, 2>);
+      if constexpr (!X && S)
+        if (l.kind == Kind::Wide) return tile(gemm_fp8_tile_kernel<X, A, B, S, 128, 256, 1, 4, true, false>);
+      return direct ? tile(gemm_fp8_tile_kernel<X, A, B, S, 128, 128, 2, 2, false, false>)
+                    : tile(gemm_fp8_tile_kernel<X, A, B, S, 128, 128, 2, 2, false, true>);
     };
-    auto any_small = [&](const Fp8GemmArgs &a, Kind kind) {
-      if (kind == Kind::Small11) return small(a, gemm_fp8_small_kernel<X, A, B, S, 1, 1, 3>, 16, 16);
-      if (kind == Kind::Small22) return small(a, gemm_fp8_small_kernel<X, A, B, S, 2, 2, 2>, 32, 32);
-      return small(a, gemm_fp8_small_kernel<X, A, B, S, 4, 2, 2>, 64, 32);
-    };
-    const Kind kind = kind_of(args.M, args.N, args.K);
-    if (kind != Kind::Tile) return any_small(args, kind);
-    if constexpr (!X && S)
-      if (aligned && tiles_of(args.M, 128) * tiles_of(args.N, 256) >= 512) {
-        // A last column of tiles that is nearly empty and costs a round of the
-        // CUs goes to the small kernel (4,001 x 4,099 x 8,200: 198 -> 160 us).
-        auto rounds = [&](int64_t N) { return tiles_of(tiles_of(args.M, 128) * tiles_of(N, 256), 512); };
-        Fp8GemmArgs a = args, edge = args;
-        const int64_t over = args.N % 256;
-        if (over > 0 && over <= 32 && blocks >= 16 && rounds(args.N - over) < rounds(args.N)) {
-          a.N -= over;
-          edge.N = over;
-          edge.B = (const char *)edge.B + a.N * edge.ldb;
-          edge.sb += a.N / kFp8Block;
-          edge.C = (char *)edge.C + a.N * 2;
-          const hipError_t e = any_small(edge, over <= 16 ? Kind::Small11 : Kind::Small22);
-          if (e != hipSuccess) return e;
-        }
-        return rows(a, 128, 256, [&](const Fp8GemmArgs &a, uint32_t tm, uint32_t tn) {
-          hipLaunchKernelGGL((gemm_fp8_tile_kernel<X, A, B, S, 128, 256, 1, 4, true, false>), dim3(tm * tn), dim3(256), 0, s, a,
-                             c_type, tm, tn, (uint32_t)blocks);
-          return hipGetLastError();
-        });
-      }
-    const int split = split_of(args.M, args.N, args.K, X);
-    const uint32_t each = (uint32_t)tiles_of(blocks, split);
-    const int parts = each ? (int)tiles_of(blocks, each) : 1;
-    const hipError_t e = rows(args, 128, 128, [&](const Fp8GemmArgs &a, uint32_t tm, uint32_t tn) {
-      auto kernel = aligned ? gemm_fp8_tile_kernel<X, A, B, S, 128, 128, 2, 2, false, false>
-                            : gemm_fp8_tile_kernel<X, A, B, S, 128, 128, 2, 2, false, true>;
-      hipLaunchKernelGGL(kernel, dim3(tm * tn, parts), dim3(256), 0, s, a, c_type, tm, tn, each);
-      return hipGetLastError();
-    });
-    if (parts == 1 || e != hipSuccess) return e;
-    const int64_t per_row = tiles_of(args.N, 4);  // at most 512 tiles are split: one launch
-    const dim3 grid((unsigned)tiles_of(args.M * per_row, 256));
+    const hipError_t e = fp8plan::for_launches(args.M, args.N, args.K, X, S, direct, hipSuccess, launch);
+    if (e != hipSuccess || parts == 1) return e;
+    const int64_t per_row = fp8plan::tiles_of(args.N, 4);  // at most 512 tiles are split: one launch
+    const dim3 grid((unsigned)fp8plan::tiles_of(args.M * per_row, 256));
     if (X) hipLaunchKernelGGL(gemm_fp8_join_kernel<float>, grid, dim3(256), 0, s, args, parts, per_row);
     else if (c_type == PREC_BF16) hipLaunchKernelGGL(gemm_fp8_join_kernel<bf16>, grid, dim3(256), 0, s, args, parts, per_row);
     else hipLaunchKernelGGL(gemm_fp8_join_kernel<f16>, grid, dim3(256), 0, s, args, parts, per_row);
