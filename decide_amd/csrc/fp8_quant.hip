@@ -124,24 +124,34 @@ __global__ __launch_bounds__(Shape::MAXT) void rms_kernel(RmsArgs a, int64_t fir
 #pragma unroll
     for (int i = 0; i < VEC; i++) w[i] = 1.0f;
     if (a.w) load<float, VEC>(a.w, c, cols, w);
-    float most = 0.0f;
-#pragma unroll
-    for (int i = 0; i < VEC; i++) {
-      v[j][i] *= w[i];
-      most = fmaxf(most, fabsf(v[j][i]));
-    }
     if (a.q) {
       // y / scale without y's own rounding: rstd, which all of a block shares,
-      // cancels, unless the block is zeros, tiny or not finite.
+      // cancels. Not so in a block whose y or h w is zeros, tiny or not finite,
+      // where rstd times either side's inverse would leave fp32's range: y itself.
+      float p[VEC], most = 0.0f;
+#pragma unroll
+      for (int i = 0; i < VEC; i++) {
+        p[i] = v[j][i] * w[i];
+        most = fmaxf(most, fabsf(p[i]));
+      }
       most = lanes_max<LANES>(most);
-      const float top = largest(a.e5m2), of_y = most * rstd;
-      const bool plain = of_y >= kLeast && of_y < INFINITY;
-      store8<VEC>((uint8_t *)a.q + row * a.ldq, c, cols, v[j], plain ? top / most : rstd * (top / kLeast), a.e5m2);
-      if (lane % LANES == 0 && c < cols) a.scale[c / kFp8Block * a.ldscale + row] = (plain ? of_y : kLeast) / top;
+      float of_y = most * rstd;
+      if (!(most >= kLeast && of_y >= kLeast && of_y < INFINITY)) {
+        most = kLeast;
+#pragma unroll
+        for (int i = 0; i < VEC; i++) {
+          p[i] = v[j][i] * rstd * w[i];
+          most = fmaxf(most, fabsf(p[i]));
+        }
+        of_y = most = lanes_max<LANES>(most);
+      }
+      const float top = largest(a.e5m2);
+      store8<VEC>((uint8_t *)a.q + row * a.ldq, c, cols, p, top / most, a.e5m2);
+      if (lane % LANES == 0 && c < cols) a.scale[c / kFp8Block * a.ldscale + row] = of_y / top;
     }
     if (a.y) {
 #pragma unroll
-      for (int i = 0; i < VEC; i++) v[j][i] *= rstd;
+      for (int i = 0; i < VEC; i++) v[j][i] = v[j][i] * w[i] * rstd;
       store<Y, VEC>((Y *)a.y + row * a.ldy, c, cols, v[j]);
     }
   }

@@ -1,12 +1,14 @@
 """The 8-bit operators on the GPU at the edges of their ranges: products of many
 rows and few columns, and of a last column of tiles that has a launch of its
-own. Bounds: fp8_reference.py."""
+own; norms of zeros and of values near the ends of fp32. Bounds: fp8_reference.py."""
 import numpy as np
 import pytest
 import torch
 
 import fp8_reference as ref
-from test_gpu_fp8_ops import TYPES, Matrix, at, check_gemm, eng, f64, ptr, scale_matrix, within  # noqa: F401
+from fp8_reference import U
+from test_gpu_fp8_ops import (TYPES, Matrix, at, check_gemm, check_quantised, eng, f64, ptr, scale_matrix,  # noqa: F401
+                              vec, within)
 
 pytestmark = pytest.mark.gpu
 
@@ -40,3 +42,42 @@ def test_last_columns_of_17_to_32(eng, M, N, K):  # noqa: F811
     """A last column of tiles of 17 to 32 outputs, in a launch of its own."""
     rng = np.random.default_rng(N)
     check_gemm(eng, rng, M, N, K, ("e5m2", "e4m3"), "bf16", pad=-K % 16, c_pad=3)
+
+
+def norm_of(eng, v, eps, qt, w=None, y=True):  # noqa: F811
+    """(y, q, scale, rstd) of the RMS norm of rows of fp32 values, and y and rstd in 64 bits."""
+    rows, cols = v.shape
+    x, Y = Matrix(rows, cols, "fp32", v), Matrix(rows, cols, "fp32")
+    Q, scale, rstd = Matrix(rows, cols, qt), scale_matrix(rows, cols), torch.empty(rows, device="cuda")
+    w = None if w is None else vec(w)
+    eng.add_rms_norm_device("fp32", "fp32", "fp32", qt, rows, cols, *at(x), None, 0, ptr(w), eps, None, 0,
+                            *(at(Y) if y else (None, 0)), *at(Q), *at(scale), ptr(rstd))
+    return Y, Q, scale, rstd, *ref.rms(x.f64(), f64(w), float(np.float32(eps)))
+
+
+@pytest.mark.parametrize("eps", [1e-5, 4e-8, 1e-8, 1e-12, 1e-20, 1e-30, 1e-38])
+@pytest.mark.parametrize("qt", ["e4m3", "e5m2"])
+def test_norm_of_zeros_and_tiny_values(eng, qt, eps):  # noqa: F811
+    """Rows and blocks of zeros give zeros with the least scale for every eps, whatever rstd = eps^-0.5 is; values so
+    small that rstd lifts them, or does not, above the least magnitude of a block keep their relative precision."""
+    rng = np.random.default_rng(11)
+    for cols in (1, 7, 100, 128, 300, 768, 2900, 9000):
+        v = rng.standard_normal((12, cols))
+        v[0] = 0.0
+        for r, size in enumerate((1e-20, 1e-25, 1e-30, 1e-33, 1e-34, 1e-35, 1e-36, 2.0 ** -100)):
+            v[1 + r] *= size
+        v[9, cols // 2:] = 0.0
+        v[10, cols // 2:] *= 1e-34
+        v[11, :cols // 2] *= 1e-37
+        Y, Q, scale, rstd, want, r64 = norm_of(eng, v, eps, qt)
+        # Squares below fp32's smallest normal lose up to half of its smallest step each, eps's sum one more.
+        rel = ref.RMS_REL + 2 * 2.0 ** -149 / np.float32(eps)
+        within(f64(rstd), r64, rel * r64, ("rstd", cols))
+        e = (rel + 2 * U) * np.abs(want) + 2.0 ** -149
+        within(Y.f64(), want, e + U * np.abs(want), ("y", cols))
+        check_quantised(Q, scale, want, e, qt, (cols, eps))
+        zeros = Q.f64()[0], Q.f64()[9, cols // 2:]
+        assert not zeros[0].any() and not zeros[1].any()
+        least = np.float32(2.0 ** -100) / np.float32(ref.MOST[qt])
+        assert (scale.f64()[:, 0] == least).all()
+        assert cols < 512 or (scale.f64()[-1, 9] == least).all()
