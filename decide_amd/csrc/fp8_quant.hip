@@ -151,7 +151,7 @@ __global__ __launch_bounds__(Shape::MAXT) void rms_kernel(RmsArgs a, int64_t fir
     }
     if (a.y) {
 #pragma unroll
-      for (int i = 0; i < VEC; i++) v[j][i] = v[j][i] * w[i] * rstd;
+      for (int i = 0; i < VEC; i++) v[j][i] = v[j][i] * rstd * w[i];
       store<Y, VEC>((Y *)a.y + row * a.ldy, c, cols, v[j]);
     }
   }

@@ -81,3 +81,37 @@ def test_norm_of_zeros_and_tiny_values(eng, qt, eps):  # noqa: F811
         least = np.float32(2.0 ** -100) / np.float32(ref.MOST[qt])
         assert (scale.f64()[:, 0] == least).all()
         assert cols < 512 or (scale.f64()[-1, 9] == least).all()
+
+
+@pytest.mark.parametrize("y", [True, False])
+def test_norm_weights_near_the_ends(eng, y):  # noqa: F811
+    """y = (h rstd) w: where h w alone would leave fp32's range, above or below, y does not; a block whose y is
+    infinite has an infinite scale, its finite rows and blocks do not see it."""
+    rng = np.random.default_rng(12)
+    for cols in (1, 7, 100, 300, 768, 2900, 9000):
+        for size, weight, eps in ((1e6, 1e34, 1e-5), (1e16, 1e30, 1e-5), (1e-25, 1e-18, 1e-38), (1e-24, 1e-20, 1e-38)):
+            v = rng.standard_normal((6, cols)) * size
+            w = weight * (0.5 + rng.random(cols))
+            Y, Q, scale, rstd, want, r64 = norm_of(eng, v, eps, "e4m3", w, y)
+            rel = ref.RMS_REL + 2 * 2.0 ** -149 / np.float32(eps)
+            within(f64(rstd), r64, rel * r64, ("rstd", cols))
+            # A row's smallest elements times rstd may be below fp32's normal range: half of its step, times w.
+            e = (rel + 2 * U) * np.abs(want) + 2.0 ** -150 * (1 + w)
+            if y:
+                within(Y.f64(), want, e + U * np.abs(want), ("y", cols, size))
+            check_quantised(Q, scale, want, e, "e4m3", (cols, size))
+    # y past fp32's range in one block: infinite there, in y and in its scale.
+    w = np.ones(300)
+    w[130] = 1e38
+    v = rng.standard_normal((5, 300))
+    v[:, 130], v[4, 130] = 10.0, 0.0
+    Y, Q, scale, rstd, want, r64 = norm_of(eng, v, 1e-5, "e4m3", w, y)
+    over = want[:, 130] > 3.5e38
+    assert over[:4].all() and not over[4]
+    assert np.array_equal(np.isinf(scale.f64()), np.array([[False] * 5, list(over), [False] * 5]))
+    for b, at_columns in enumerate((slice(0, 128), slice(128, 256), slice(256, 300))):
+        for r in range(5):
+            stands = Q.f64()[r, at_columns] * np.float64(scale.f64()[b, r]) if not (b == 1 and over[r]) else None
+            assert stands is None or np.abs(stands - want[r, at_columns]).max() <= np.abs(want[r, at_columns]).max() / 16
+    if y:
+        assert np.array_equal(np.isinf(Y.f64()), np.abs(want) > 3.5e38)
