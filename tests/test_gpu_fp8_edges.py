@@ -115,3 +115,120 @@ def test_norm_weights_near_the_ends(eng, y):  # noqa: F811
             assert stands is None or np.abs(stands - want[r, at_columns]).max() <= np.abs(want[r, at_columns]).max() / 16
     if y:
         assert np.array_equal(np.isinf(Y.f64()), np.abs(want) > 3.5e38)
+
+
+NAN8 = 0x7F  # a NaN of both 8-bit types
+
+
+def poisoned(rng, rows, K, dtype, block_rows, lead, pad):
+    """An operand and its scales, every byte beside them a NaN."""
+    v = rng.standard_normal((rows, K)) * np.exp2(rng.integers(-6, 3, (rows, K)))
+    m, s = Matrix(rows, K, dtype, lead=lead, pad=pad), scale_matrix(rows, K, block_rows, pad)
+    m.bytes.fill_(NAN8)
+    m.raw().copy_(torch.from_numpy(v).cuda().float().to(TYPES[dtype]).view(m.bits))
+    s.bytes.view(torch.float32).fill_(float("nan"))
+    s.view.copy_(torch.from_numpy(np.exp(rng.standard_normal(tuple(s.view.shape)) - 4)))
+    return m, s
+
+
+# A size for each kernel: 16 x 16, 32 x 32, 64 x 32, 128 x 128 and 128 x 256 outputs, and one split along K.
+@pytest.mark.parametrize("M,N,K", [(M, N, K) for M, N in ((40, 50), (500, 400), (64, 8200), (1000, 900), (32641, 385))
+                                   for K in (1, 15, 17, 129, 260, 1143)] + [(500, 400, 9001)])
+def test_nothing_behind_a_row_takes_part(eng, M, N, K):  # noqa: F811
+    """NaNs fill every byte that belongs to no element, of operands and scales. A NaN, an infinity and an infinite
+    scale reach their own rows and columns and no others, in every type of C."""
+    rng = np.random.default_rng(M + K)
+    wide = M > 30000
+    for k, ct in enumerate(("bf16", "fp16") if wide else ("bf16", "fp16", "fp32")):
+        for lead, pad in ((0, -K % 16), (16, -K % 16 + 16), (1, 3)):
+            if wide and lead != 16 * k:  # the 128 x 256 kernel takes aligned rows alone
+                continue
+            b_rows = 128 if wide or (lead + k) % 2 else 1
+            a, sa = poisoned(rng, M, K, "e5m2", 1, lead, pad)
+            b, sb = poisoned(rng, N, K, "e4m3", b_rows, lead, pad)
+            a.raw()[5, K - 1], a.raw()[12, 0], b.raw()[7, K // 2] = 0x7C, 0x7E, 0x7F  # inf, NaN, NaN
+            sa.view[0, 20] = float("inf")
+            b.raw()[30] = 0
+            c = Matrix(M, N, ct, lead=lead, pad=pad)
+            work = torch.empty(max(1, eng.gemm_fp8_workspace(M, N, K)), dtype=torch.uint8, device="cuda")
+            eng.gemm_fp8_device("e5m2", "e4m3", ct, M, N, K, *at(a), *at(sa), *at(b), b_rows, *at(sb), *at(c), False,
+                                ptr(work), work.numel())
+            what, got = (M, N, K, ct, lead, pad), c.f64()
+            bad = np.zeros((M, N), bool)
+            bad[[5, 12, 20]], bad[:, 7] = True, True
+            assert np.array_equal(~np.isfinite(got), bad), what
+            assert np.isnan(got[12]).all() and np.isnan(got[:, 7]).all() and np.isnan(got[[5, 20], 30]).all(), what
+            assert c.untouched_outside(), what
+            if not wide or K < 300:
+                va, vs = a.f64(), sa.f64()
+                va[[5, 12]], vs[0, 20] = 0.0, 0.0
+                vb = b.f64()
+                vb[7] = 0.0
+                want, terms = ref.gemm(va, vs, vb, sb.f64(), b_rows)
+                bound = ref.gemm_bound(terms, ref.blocks(K), want, ct)
+                within(np.where(bad, 0.0, got), np.where(bad, 0.0, want), bound, what)
+
+
+@pytest.mark.parametrize("dtype", ["e4m3", "e5m2"])
+@pytest.mark.parametrize("ct", ["fp32", "bf16", "fp16"])
+def test_every_value_of_a_type(eng, dtype, ct):  # noqa: F811
+    """Each 8-bit value, subnormals among them, times 1 (and times the least subnormal) is itself: it has at most four
+    significant bits."""
+    codes = torch.arange(256, dtype=torch.uint8, device="cuda")
+    codes = codes[torch.isfinite(codes.view(TYPES[dtype]).float())]
+    n = codes.numel()
+    for M in (n, 4 * n, 40 * n):
+        a = codes.repeat(M // n)[:, None].expand(M, 128).contiguous()
+        eye = torch.zeros(128, 128, dtype=torch.uint8, device="cuda")
+        ones = torch.tensor([1.0], device="cuda").to(TYPES[dtype]).view(torch.uint8)
+        for code, by in ((ones, 1.0), (torch.tensor([1], dtype=torch.uint8), 2.0 ** (-9 if dtype == "e4m3" else -16))):
+            b = eye.clone()
+            b.fill_diagonal_(int(code))
+            sa, sb = torch.ones(1, M, device="cuda"), torch.full((1, 128), 1 / by, device="cuda")
+            c = torch.empty(M, 128, dtype=TYPES[ct], device="cuda")
+            work = torch.empty(max(1, eng.gemm_fp8_workspace(M, 128, 128)), dtype=torch.uint8, device="cuda")
+            eng.gemm_fp8_device(dtype, dtype, ct, M, 128, 128, ptr(a), 128, ptr(sa), M, ptr(b), 128, 1, ptr(sb), 128, ptr(c),
+                                128, False, ptr(work), work.numel())
+            want = codes.view(TYPES[dtype]).float().repeat(M // n)[:, None].expand(M, 128).to(TYPES[ct])
+            assert torch.equal(c.float(), want.float()), (dtype, ct, M, by)
+
+
+def test_more_rows_than_a_launch_takes(eng):  # noqa: F811
+    """2^22 tiles of 128 rows and more, 2^20 workgroups of rows of the norm, 2^20 tiles of the quantiser."""
+    M, K = (1 << 29) + 200, 16
+    for lda, M in ((16, M), (1, M)):
+        K = lda
+        a = torch.full((M, lda), 0x38, dtype=torch.uint8, device="cuda")  # 1
+        b, sb = torch.full((1, 16), 0x38, dtype=torch.uint8, device="cuda"), torch.ones(1, 1, device="cuda")
+        sa = (torch.arange(M, dtype=torch.int32, device="cuda") % 251).float()  # at most 8 bits
+        c = torch.zeros(M, dtype=torch.bfloat16, device="cuda")
+        eng.gemm_fp8_device("e4m3", "e4m3", "bf16", M, 1, K, ptr(a), lda, ptr(sa), M, ptr(b), 16, 128, ptr(sb), 1, ptr(c), 1)
+        torch.cuda.synchronize()
+        del a
+        for r in range(0, M, 1 << 26):
+            assert torch.equal(c[r:r + (1 << 26)].float(), sa[r:r + (1 << 26)] * K), (lda, r)
+        del c, sa
+    rows = (1 << 20) * 32 + 41
+    x = torch.randn(rows, 8, device="cuda").bfloat16()
+    q, s = torch.zeros(rows, 8, dtype=torch.uint8, device="cuda"), torch.zeros(rows, device="cuda")
+    y = torch.zeros(rows, 8, dtype=torch.bfloat16, device="cuda")
+    eng.add_rms_norm_device("bf16", "bf16", "bf16", "e4m3", rows, 8, ptr(x), 8, None, 0, None, 1e-5, None, 0, ptr(y), 8,
+                            ptr(q), 8, ptr(s), rows)
+    want = x.float() / (x.float().square().mean(1, keepdim=True) + 1e-5).sqrt()
+    rel = 2.0 ** -8 + 2.0 ** -18  # bf16's rounding; fp32's of both sides
+    assert bool(((y.float() - want).abs() <= want.abs() * rel + 2.0 ** -60).all())
+    off = (q.view(torch.float8_e4m3fn).float() * s[:, None] - want).abs()
+    assert bool((off <= want.abs() * (2.0 ** -4 + 2.0 ** -18) + s[:, None] * 2.0 ** -10).all())
+    del x, y, q, s, want, off
+    rows = (1 << 20) * 128 + 77
+    x = torch.randn(rows, 1, device="cuda")
+    q, qt = torch.zeros(rows, dtype=torch.uint8, device="cuda"), torch.zeros(rows, dtype=torch.uint8, device="cuda")
+    nb = ref.blocks(rows)
+    s, st = torch.zeros(nb, device="cuda"), torch.zeros(nb, device="cuda")
+    eng.quantize_blocks_device("fp32", "e4m3", rows, 1, 128, ptr(x), 1, ptr(q), 1, ptr(s), nb, ptr(qt), rows, ptr(st), 1)
+    assert torch.equal(q, qt) and torch.equal(s, st)
+    tall = torch.zeros(nb * 128, device="cuda")
+    tall[:rows] = x[:, 0]
+    assert torch.equal(s, (tall.view(nb, 128).abs().amax(1).double() / 448).float())
+    off = (q.view(torch.float8_e4m3fn).float() * s.repeat_interleave(128)[:rows] - x[:, 0]).abs()
+    assert bool((off <= x[:, 0].abs() * (2.0 ** -4 + 2.0 ** -20) + s.repeat_interleave(128)[:rows] * 2.0 ** -10).all())
