@@ -36,7 +36,7 @@ int dn_layer_norm_device(dn_ctx *c, int x_type, int y_type, int64_t rows, int co
   a.mean = d_mean;
   a.rstd = d_rstd;
   return device_call(c, "layer_norm", [&] { return blockchk::norm(x_type, y_type, a); },
-             [&] { return launch_norm(x_type, y_type, a, c->stream); });
+                     [&] { return launch_norm(x_type, y_type, a, c->stream); });
 }
 
 int64_t dn_norm_backward_workspace(int64_t rows, int cols) {
@@ -65,8 +65,8 @@ int dn_layer_norm_backward_device(dn_ctx *c, int dy_type, int x_type, int64_t ro
   a.accumulate = accumulate ? 1 : 0;
   a.work = (float *)d_work;
   return device_call(c, "layer_norm_backward",
-             [&] { return blockchk::norm_grad(dy_type, x_type, a, work_floats(rows, cols), work_bytes); },
-             [&] { return launch_norm_grad(dy_type, x_type, a, c->stream); });
+                     [&] { return blockchk::norm_grad(dy_type, x_type, a, work_floats(rows, cols), work_bytes); },
+                     [&] { return launch_norm_grad(dy_type, x_type, a, c->stream); });
 }
 
 int dn_dropout_device(dn_ctx *c, int x_type, int y_type, int64_t rows, int64_t cols, const void *d_x, int64_t ldx,
@@ -82,7 +82,7 @@ int dn_dropout_device(dn_ctx *c, int x_type, int y_type, int64_t rows, int64_t c
   a.y = d_y;
   a.ldy = ldy;
   return device_call(c, "dropout", [&] { return blockchk::dropout(x_type, y_type, p, seed, offset, &a); },
-             [&] { return launch_dropout(x_type, y_type, a, c->stream); });
+                     [&] { return launch_dropout(x_type, y_type, a, c->stream); });
 }
 
 int dn_dropout_add_norm_device(dn_ctx *c, int x_type, int stream_type, int y_type, int64_t rows, int cols,
@@ -106,8 +106,8 @@ int dn_dropout_add_norm_device(dn_ctx *c, int x_type, int stream_type, int y_typ
   a.mean = d_mean;
   a.rstd = d_rstd;
   return device_call(c, "dropout_add_norm",
-             [&] { return blockchk::boundary(x_type, stream_type, y_type, p, seed, offset, &a); },
-             [&] { return launch_boundary(x_type, stream_type, y_type, a, c->stream); });
+                     [&] { return blockchk::boundary(x_type, stream_type, y_type, p, seed, offset, &a); },
+                     [&] { return launch_boundary(x_type, stream_type, y_type, a, c->stream); });
 }
 
 int dn_dropout_add_norm_backward_device(dn_ctx *c, int dy_type, int stream_type, int dx_type, int64_t rows, int cols,
@@ -137,11 +137,11 @@ int dn_dropout_add_norm_backward_device(dn_ctx *c, int dy_type, int stream_type,
   a.accumulate = accumulate ? 1 : 0;
   a.work = (float *)d_work;
   return device_call(c, "dropout_add_norm_backward",
-             [&] {
-               return blockchk::boundary_grad(dy_type, stream_type, dx_type, p, seed, offset, &a,
-                                              work_floats(rows, cols), work_bytes);
-             },
-             [&] { return launch_boundary_grad(dy_type, stream_type, dx_type, a, c->stream); });
+                     [&] {
+                       return blockchk::boundary_grad(dy_type, stream_type, dx_type, p, seed, offset, &a,
+                                                      work_floats(rows, cols), work_bytes);
+                     },
+                     [&] { return launch_boundary_grad(dy_type, stream_type, dx_type, a, c->stream); });
 }
 
 }  // extern "C"
