@@ -153,7 +153,7 @@ struct TileAt {
 // end is its padding or the next row (nothing past the array's last chunk), and
 // the last block's is cleared in LDS before it is multiplied. RAGGED: rows of any
 // alignment, through registers, whose unaligned loads bound it (4,001 x 4,099 x
-// 8,200 410 us, aligned 160; 4,096 x 768 x 768 16 and 9).
+// 8,200 406 us, aligned 161; 4,096 x 768 x 768 16 and 8).
 //
 // B is the instruction's first operand, its rows dealt to the tiles of a wave so
 // that a lane holds runs of eight consecutive columns of C: 16 bytes of a 16-bit
@@ -161,15 +161,17 @@ struct TileAt {
 //
 // ONE_B: B has one slot, since a wave holds a block's B in registers before the
 // next one's is needed: two workgroups of 128 x 256 tiles fit a CU's LDS, each of
-// which computes while the other waits (32,768 x 2,304 x 768: 90 us; 256 x 256 by
-// eight waves with two slots 99, 128 x 128 104; 8,192 cubed 494, 496, 557).
+// which computes while the other waits (32,768 x 2,304 x 768: 90 us, 128 x 128 96;
+// 8,192 cubed 499 and 559).
 //
-// Bound by power: at 8,192 cubed (2.2 PFLOP/s; a library product without block
-// scales 2.7) the matrix cores are 55% busy at 1.84 GHz, LDS 25%, no bank
-// conflicts. At K = 768 the tiles without their stores take 63 us and the stores
-// alone 36, and neither staggered starts nor more loads in flight overlap them.
-// EXACT: the vector unit, which widens the operands, and the matrix cores share a
-// wave's issue: 60% and 45% busy (1.1 PFLOP/s at 8,192 cubed).
+// At 8,192 cubed (495 us, 2.2 PFLOP/s; a library product without block scales 2.7)
+// bound by power: the matrix cores are 63% busy, LDS 28%, no bank conflicts, and
+// launches of equal cycles take 482 us at 1.8 GHz and 575 at 1.5. At K = 768
+// (32,768 x 2,304, 1.3 PFLOP/s) the matrix cores are 38% busy: the tiles without
+// their stores take 58 us and the stores alone 31, which overlap only between a
+// CU's two workgroups, and the last of 4.5 rounds leaves half of the places empty.
+// EXACT (928 us at 8,192 cubed, 1.2 PFLOP/s): the vector unit, which widens the
+// operands, and the matrix cores share a wave's issue: 50% and 60% busy.
 template <bool EXACT, bool E5A, bool E5B, bool SQUARE, int BM, int BN, int WGM, int WGN, bool ONE_B, bool RAGGED>
 __global__ __launch_bounds__(64 * WGM * WGN, 2) void gemm_fp8_tile_kernel(Fp8GemmArgs g, int c_type, uint32_t tiles_m,
                                                                          uint32_t tiles_n, uint32_t each) {

@@ -19,23 +19,23 @@ enum class Kind { Small11, Small22, Small42, Tile, Wide };
 inline int rows_of(Kind k) { return k == Kind::Small11 ? 16 : k == Kind::Small22 ? 32 : k == Kind::Small42 ? 64 : 128; }
 inline int cols_of(Kind k) { return k == Kind::Small11 ? 16 : k == Kind::Tile ? 128 : k == Kind::Wide ? 256 : 32; }
 
-// The kernel of a product of these sizes. Times in us on the GPU, bf16 C with
-// 128 x 128 scales unless said:
+// The kernel of a product of these sizes. Median times in us of the kernel alone,
+// bf16 C with 128 x 128 scales unless said:
 //                          16 x 16  32 x 32  64 x 32  128 x 128  128 x 256
-//   1 x 8,192 x 8,192        14.0     13.6     17.2      37.8
-//   16 x 8,192 x 4,096       10.8      9.8     11.5      21.1
-//   64 x 8,192 x 4,096       33.2     22.2     16.8      22.4
-//   100 x 768 x 768           4.4      4.6      5.7       7.3
-//   200 x 768 x 2,304         9.6      7.9     10.0      13.9
-//   512 x 768 x 768           8.9      7.2      6.0       7.9
-//   512 x 2,304 x 768        21.8     14.4     14.2       8.3
-//   4,096 x 2,304 x 768                                  18.6       19.6
-//   12,288 x 768 x 2,304                                 33.9       34.3
-//   4,096 x 4,096 x 4,096                                75.1       67.4
-//   32,768 x 2,304 x 768                                 103.8      90.2
+//   1 x 8,192 x 8,192        13.4     13.9     16.4      38.6
+//   16 x 8,192 x 4,096       10.6      9.6     11.1      21.1
+//   64 x 8,192 x 4,096       31.8     19.7     15.2      21.8
+//   100 x 768 x 768           4.2      4.6      5.6       7.3
+//   200 x 768 x 2,304         9.6      7.8      9.8      13.8
+//   512 x 768 x 768           9.1      7.0      6.0       7.8
+//   512 x 2,304 x 768        21.8     14.4     14.2       8.4
+//   4,096 x 2,304 x 768                                  18.6       20.0
+//   12,288 x 768 x 2,304                                 34.6       37.2
+//   4,096 x 4,096 x 4,096                                74.0       72.4
+//   32,768 x 2,304 x 768                                 96.3       90.0
 // The small kernel as long as one round of the CUs holds its tiles (its waves
 // share K, so that past 64 rows a long K goes to tiles whose parts workgroups
-// share: 384 x 384 x 12,288 into fp32 27.0 and 18.5).
+// share: 384 x 384 x 12,288 into fp32 39.4 and 17.6 a call).
 inline Kind kind_of(int64_t M, int64_t N, int64_t K) {
   if (M > 64 && K > 64 * 128) return Kind::Tile;
   if (tiles_of(M, 16) * tiles_of(N, 16) <= 384) return Kind::Small11;
@@ -47,8 +47,8 @@ inline Kind kind_of(int64_t M, int64_t N, int64_t K) {
 // Workgroups that share a 128 x 128 tile's blocks along K, by what they cost: a
 // block 0.65 us (EXACT 1.2), half as much again for two workgroups on a CU, and
 // the join 7 us (a launch) and the partial sums' bytes (2,304 x 768 x 12,288
-// into fp32: one 123 us, two 75, four 65; 512 x 4,096 x 4,096 into bf16: one 23,
-// two 25, four 28).
+// into fp32: one 125 us, two 74, three 78, four 67; 512 x 4,096 x 4,096 into bf16:
+// one 22, two 23, four 25).
 inline int split_of(int64_t M, int64_t N, int64_t K, bool exact) {
   if (kind_of(M, N, K) != Kind::Tile) return 1;
   const int64_t tiles = tiles_of(M, 128) * tiles_of(N, 128), blocks = tiles_of(K, 128);
@@ -106,12 +106,15 @@ E for_launches(int64_t M, int64_t N, int64_t K, bool exact, bool square, bool di
   if (kind != Kind::Tile) return rows(kind, 0, N, (uint32_t)blocks, 1);
   if (!exact && square && direct && tiles_of(M, 128) * tiles_of(N, 256) >= 512) {
     // A last column of tiles that is nearly empty and costs a round of the
-    // CUs goes to the small kernel: in one launch and in two, us,
+    // CUs goes to the small kernel: in one launch and in two, us a call,
     //   4,001 x 4,099 x 8,200    204  169     8,065 x 2,051 x 2,064     62   51
     //   4,001 x 4,128 x 8,192    165  144     8,065 x 2,080 x 2,064     62   52
     //   4,001 x 4,128 x 2,048     49   43    16,257 x 1,056 x 4,096     94   87
-    // Where it is the only column, one launch stays (in the small kernel and in
-    // this one: 65,536 x 32 x 2,048 47 and 38, 70,000 x 1 x 2,048 37 and 51).
+    // Below 16 blocks of K and past 32 columns it would gain at some sizes too
+    // (4,001 x 4,112 x 768 27 and 23, 4,001 x 4,160 x 2,048 50 and 43) and at some
+    // not (16,257 x 1,056 x 768 26 and 26, 32,641 x 273 x 1,536 27 and 27). Where
+    // it is the only column, one launch stays (in the small kernel and in this
+    // one: 65,536 x 32 x 2,048 47 and 38, 70,000 x 1 x 2,048 37 and 51).
     auto rounds = [&](int64_t cols) { return tiles_of(tiles_of(M, 128) * tiles_of(cols, 256), 512); };
     int64_t cols = N;
     const int64_t over = N % 256;

@@ -128,6 +128,7 @@ def test_direct_loads(plan):
     top = 1 << 23
     assert plan.takes_direct(1 << 20, top, (1 << 13) - 1, top) and 255 * top + (top - 128) + 7 * 16 + 16 <= 1 << 31
     for p, ld, ld_scale, K in ((8, 16, 1, 128), (16, 24, 1, 128), (16, top + 16, 1, 128), (16, top, 1, top + 1),
-                               (16, -16, 1, 128), (16, 1024, 1 << 28, 256), (16, 1024, (1 << 28) + 1, 256), (16, top, 1 << 13, top)):
+                               (16, -16, 1, 128), (16, 1024, 1 << 28, 256), (16, 1024, (1 << 28) + 1, 256),
+                               (16, top, 1 << 13, top)):
         assert not plan.takes_direct(p, ld, ld_scale, K), (p, ld, ld_scale, K)
     assert plan.takes_direct(16, 1024, 1 << 40, 128)  # a single block: its stride is any number

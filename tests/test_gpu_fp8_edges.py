@@ -111,8 +111,10 @@ def test_norm_weights_near_the_ends(eng, y):  # noqa: F811
     assert np.array_equal(np.isinf(scale.f64()), np.array([[False] * 5, list(over), [False] * 5]))
     for b, at_columns in enumerate((slice(0, 128), slice(128, 256), slice(256, 300))):
         for r in range(5):
-            stands = Q.f64()[r, at_columns] * np.float64(scale.f64()[b, r]) if not (b == 1 and over[r]) else None
-            assert stands is None or np.abs(stands - want[r, at_columns]).max() <= np.abs(want[r, at_columns]).max() / 16
+            if b == 1 and over[r]:
+                continue
+            stands, wanted = Q.f64()[r, at_columns] * scale.f64()[b, r], want[r, at_columns]
+            assert np.abs(stands - wanted).max() <= np.abs(wanted).max() / 16
     if y:
         assert np.array_equal(np.isinf(Y.f64()), np.abs(want) > 3.5e38)
 
@@ -187,8 +189,8 @@ def test_every_value_of_a_type(eng, dtype, ct):  # noqa: F811
             sa, sb = torch.ones(1, M, device="cuda"), torch.full((1, 128), 1 / by, device="cuda")
             c = torch.empty(M, 128, dtype=TYPES[ct], device="cuda")
             work = torch.empty(max(1, eng.gemm_fp8_workspace(M, 128, 128)), dtype=torch.uint8, device="cuda")
-            eng.gemm_fp8_device(dtype, dtype, ct, M, 128, 128, ptr(a), 128, ptr(sa), M, ptr(b), 128, 1, ptr(sb), 128, ptr(c),
-                                128, False, ptr(work), work.numel())
+            eng.gemm_fp8_device(dtype, dtype, ct, M, 128, 128, ptr(a), 128, ptr(sa), M, ptr(b), 128, 1, ptr(sb), 128,
+                                ptr(c), 128, False, ptr(work), work.numel())
             want = codes.view(TYPES[dtype]).float().repeat(M // n)[:, None].expand(M, 128).to(TYPES[ct])
             assert torch.equal(c.float(), want.float()), (dtype, ct, M, by)
 
@@ -202,7 +204,8 @@ def test_more_rows_than_a_launch_takes(eng):  # noqa: F811
         b, sb = torch.full((1, 16), 0x38, dtype=torch.uint8, device="cuda"), torch.ones(1, 1, device="cuda")
         sa = (torch.arange(M, dtype=torch.int32, device="cuda") % 251).float()  # at most 8 bits
         c = torch.zeros(M, dtype=torch.bfloat16, device="cuda")
-        eng.gemm_fp8_device("e4m3", "e4m3", "bf16", M, 1, K, ptr(a), lda, ptr(sa), M, ptr(b), 16, 128, ptr(sb), 1, ptr(c), 1)
+        eng.gemm_fp8_device("e4m3", "e4m3", "bf16", M, 1, K, ptr(a), lda, ptr(sa), M, ptr(b), 16, 128, ptr(sb), 1,
+                            ptr(c), 1)
         torch.cuda.synchronize()
         del a
         for r in range(0, M, 1 << 26):
@@ -225,7 +228,8 @@ def test_more_rows_than_a_launch_takes(eng):  # noqa: F811
     q, qt = torch.zeros(rows, dtype=torch.uint8, device="cuda"), torch.zeros(rows, dtype=torch.uint8, device="cuda")
     nb = ref.blocks(rows)
     s, st = torch.zeros(nb, device="cuda"), torch.zeros(nb, device="cuda")
-    eng.quantize_blocks_device("fp32", "e4m3", rows, 1, 128, ptr(x), 1, ptr(q), 1, ptr(s), nb, ptr(qt), rows, ptr(st), 1)
+    eng.quantize_blocks_device("fp32", "e4m3", rows, 1, 128, ptr(x), 1, ptr(q), 1, ptr(s), nb, ptr(qt), rows, ptr(st),
+                               1)
     assert torch.equal(q, qt) and torch.equal(s, st)
     tall = torch.zeros(nb * 128, device="cuda")
     tall[:rows] = x[:, 0]
