@@ -5,10 +5,12 @@ import numpy as np
 import pytest
 import torch
 
+import block_reference as block
 import fp8_reference as ref
+from fp8_bounds import gemm_bound
 from fp8_reference import U
-from test_gpu_fp8_ops import (TYPES, Matrix, at, check_gemm, check_quantised, eng, f64, ptr, scale_matrix,  # noqa: F401
-                              vec, within)
+from test_gpu_fp8_ops import (GEMM_TYPES, TYPES, Matrix, at, check_gemm, check_quantised, eng, f64,  # noqa: F401
+                              ptr, scale_matrix, vec, within)
 
 pytestmark = pytest.mark.gpu
 
@@ -166,8 +168,8 @@ def test_nothing_behind_a_row_takes_part(eng, M, N, K):  # noqa: F811
                 va[[5, 12]], vs[0, 20] = 0.0, 0.0
                 vb = b.f64()
                 vb[7] = 0.0
-                want, terms = ref.gemm(va, vs, vb, sb.f64(), b_rows)
-                bound = ref.gemm_bound(terms, ref.blocks(K), want, ct)
+                want = ref.gemm(va, vs, vb, sb.f64(), b_rows)[0]
+                bound = gemm_bound(va, vs, vb, sb.f64(), b_rows, ("e5m2", "e4m3"), want, ct)
                 within(np.where(bad, 0.0, got), np.where(bad, 0.0, want), bound, what)
 
 
@@ -236,3 +238,32 @@ def test_more_rows_than_a_launch_takes(eng):  # noqa: F811
     assert torch.equal(s, (tall.view(nb, 128).abs().amax(1).double() / 448).float())
     off = (q.view(torch.float8_e4m3fn).float() * s.repeat_interleave(128)[:rows] - x[:, 0]).abs()
     assert bool((off <= x[:, 0].abs() * (2.0 ** -4 + 2.0 ** -20) + s.repeat_interleave(128)[:rows] * 2.0 ** -10).all())
+
+
+@pytest.mark.parametrize("types", GEMM_TYPES)
+@pytest.mark.parametrize("M,N", [(300, 200), (1500, 776)])
+def test_subnormal_operands(eng, types, M, N):  # noqa: F811
+    """Products of subnormals by large values beside smaller ones: an fp32 C keeps fp32's bits, a 16-bit C the 8-bit
+    instruction's, whose cut lies higher for them, and stays within 2^-7 (e5m2 alone: 2^-8) of the terms' magnitudes."""
+    rng = np.random.default_rng(M)
+    worst = 7 * 2.0 ** -10 if "e4m3" in types else 7 * 2.0 ** -11
+    for K in (2, 3, 8, 9, 40, 300):
+        pair = []
+        for rows, t in ((M, types[0]), (N, types[1])):
+            low, high = (-9, 8) if t == "e4m3" else (-16, 14)
+            v = rng.choice([-1.0, 1.0], (rows, K)) * np.exp2(rng.uniform(low, high, (rows, K)))
+            v[rng.random((rows, K)) < 0.5] *= 2.0 ** low  # half of them subnormal or zero
+            s = scale_matrix(rows, K)
+            s.view.copy_(torch.from_numpy(np.exp2(rng.integers(-8, -4, tuple(s.view.shape)) - (high - 8.0))))
+            pair += [Matrix(rows, K, t, v, pad=-K % 16), s]
+        a, sa, b, sb = pair
+        want, terms = ref.gemm(a.f64(), sa.f64(), b.f64(), sb.f64(), 1)
+        for ct in ("fp32", "bf16", "fp16"):
+            c = Matrix(M, N, ct)
+            work = torch.empty(max(1, eng.gemm_fp8_workspace(M, N, K)), dtype=torch.uint8, device="cuda")
+            eng.gemm_fp8_device(*types, ct, M, N, K, *at(a), *at(sa), *at(b), 1, *at(sb), *at(c), False, ptr(work),
+                                work.numel())
+            within(c.f64(), want, gemm_bound(a.f64(), sa.f64(), b.f64(), sb.f64(), 1, types, want, ct), (K, ct))
+            if ct != "fp32":  # as decide_hip.h says it
+                e = (worst + 2.0 ** -15) * terms
+                within(c.f64(), want, e + block.rounding(np.abs(want) + e, ct), (K, ct))
